@@ -601,6 +601,83 @@ void *sparse_amd_dvec_f64_member_ptr(struct sparse_amd_group *g, const struct sp
 int sparse_amd_dcsr_f64_smvm(struct sparse_amd_group *g, struct sparse_amd_dvec_f64 *y,
                              const struct sparse_amd_dcsr_f64 *A, const struct sparse_amd_dvec_f64 *x);
 
+/* ------------------------------- (7) token records: products of a language model's sparse matrices
+ * No counterpart in the reference.  Neighbours of mono (S/mono.fut:95: one stored element per row, col_idx[n] and vals[n]) and of
+ * smm for the records a language model makes anew at every step, given by their column indices alone:
+ *   - a lookup is a mono record times a panel: n token ids (col_idx), optional values f[n], one scale s for all;
+ *   - a routing is a record of K elements per row: each token's K chosen experts.  `route` gives every choice a place such
+ *     that an expert's places lie side by side, in the order of the batch; dispatch and combine are the products with that
+ *     permutation and with its weighted transpose, experts the product with the block-diagonal matrix of the experts' blocks.
+ * Conventions of this group, where they differ from the rest of this header:
+ *   - arguments are plain device pointers; a panel of rows has a row stride (`ld...`, in elements) of at least its width and
+ *     no alignment beyond its elements';
+ *   - every call names the HIP stream it runs on (NULL: the null stream) and touches neither the context's stream nor its
+ *     memory: it allocates nothing, never waits, keeps nothing between calls, and may be captured into a graph.  What needs
+ *     a workspace takes it as an argument (256-byte aligned, at least ..._workspace bytes, free for other use when the
+ *     stream has passed the call; contents do not matter).  The calling thread's current device is left as it was;
+ *   - `type` is the element type of the panels: SPARSE_AMD_F32, SPARSE_AMD_F16, SPARSE_AMD_BF16 (experts...: the 16-bit ones).
+ *     Sums are held in 32 bits and rounded once; values, weights and their gradients are 32-bit floats;
+ *   - indices that come in have `id_bits` = 32 or 64 bits.  An id outside 0 .. V-1, or an expert outside 0 .. X-1, selects
+ *     nothing: a row of zeros, no place (pos = -1), no gradient;
+ *   - results are the same bits on every call with the same arguments;
+ *   - a result may not overlap another result or an argument.
+ * Errors: as everywhere in this header (non-zero, text in futhark_context_get_error); nothing is launched then. */
+#define SPARSE_AMD_F32 0
+#define SPARSE_AMD_F16 1
+#define SPARSE_AMD_BF16 2
+/* y[i] = scale vals[i] table[ids[i]], i < n; vals may be NULL (ones). */
+int sparse_amd_tokens_lookup(struct futhark_context *ctx, void *stream, int type, void *y, int64_t ldy, const void *table,
+                             int64_t V, int64_t D, int64_t ldt, const void *ids, int id_bits, int64_t n,
+                             const float *vals, float scale);
+/* dvals[i] = scale <dy[i], table[ids[i]]>: lookup's gradient by vals. */
+int sparse_amd_tokens_lookup_dots(struct futhark_context *ctx, void *stream, int type, float *dvals, const void *dy,
+                                  int64_t ldy, const void *table, int64_t V, int64_t D, int64_t ldt, const void *ids,
+                                  int id_bits, int64_t n, float scale);
+/* dtable[v] = sum over i with ids[i] = v of scale vals[i] dy[i], added in the order of i: lookup's gradient by the table.
+ * accumulate = 0: every row of dtable is written (zeros where no id names it); else the sums are added to dtable, and rows
+ * no id names are not touched.  out_type: type or SPARSE_AMD_F32.  V and n are at most 2^31 - 2. */
+int sparse_amd_tokens_lookup_grad(struct futhark_context *ctx, void *stream, int type, int out_type, int accumulate,
+                                  void *dtable, int64_t V, int64_t D, int64_t ldt, const void *dy, int64_t ldy,
+                                  const void *ids, int id_bits, int64_t n, const float *vals, float scale, void *work,
+                                  int64_t work_bytes);
+int64_t sparse_amd_tokens_lookup_grad_workspace(int type, int64_t n, int64_t V, int64_t D);
+/* chosen[n], n = tokens * K: the experts of all tokens, X <= 1024 experts.  pos[i] = place of choice i or -1; src[p] = the
+ * choice at place p, -1 behind the last; offsets[X + 1]: expert e's places are offsets[e] .. offsets[e + 1] - 1.  The same
+ * expert twice in a token is two choices. */
+int sparse_amd_tokens_route(struct futhark_context *ctx, void *stream, const void *chosen, int id_bits, int64_t n, int64_t X,
+                            int32_t *pos, int32_t *src, int32_t *offsets, void *work, int64_t work_bytes);
+int64_t sparse_amd_tokens_route_workspace(int64_t n, int64_t X);
+/* xs[pos[t, j]] = weights[t, j] x[t], t < n, j < K; weights may be NULL (ones).  Rows of xs without a choice are left as
+ * they are.  Also the gradient of combine without weights. */
+int sparse_amd_tokens_dispatch(struct futhark_context *ctx, void *stream, int type, void *xs, int64_t ldxs, int64_t slots,
+                               const void *x, int64_t ldx, int64_t n, int64_t D, int64_t K, const int32_t *pos,
+                               const float *weights);
+/* y[t] = sum over j of weights[t, j] ys[pos[t, j]], in the order of j; weights may be NULL (ones).  A token without a place
+ * has a row of zeros; rows of ys without a choice are not read.  Also the gradient of dispatch. */
+int sparse_amd_tokens_combine(struct futhark_context *ctx, void *stream, int type, void *y, int64_t ldy, const void *ys,
+                              int64_t ldys, int64_t slots, int64_t n, int64_t D, int64_t K, const int32_t *pos,
+                              const float *weights);
+/* combine's gradient: dys[pos[t, j]] = weights[t, j] dy[t] (rows without a choice are left as they are) and
+ * dweights[t, j] = <dy[t], ys[pos[t, j]]> (0 where there is no place). */
+int sparse_amd_tokens_combine_grad(struct futhark_context *ctx, void *stream, int type, void *dys, int64_t lddys,
+                                   float *dweights, const void *dy, int64_t lddy, const void *ys, int64_t ldys,
+                                   int64_t slots, int64_t n, int64_t D, int64_t K, const int32_t *pos,
+                                   const float *weights);
+/* ys[r] = w[e] xs[r] for the rows r = offsets[e] .. offsets[e + 1] - 1 of every expert e; w[e] is F x D with rows `ldw` apart, the
+ * blocks `blockw` apart.  Rows from offsets[X] on are neither read nor written. */
+int sparse_amd_tokens_experts(struct futhark_context *ctx, void *stream, int type, void *ys, int64_t ldy, const void *xs,
+                              int64_t ldx, int64_t rows, const void *w, int64_t X, int64_t F, int64_t D, int64_t ldw,
+                              int64_t blockw, const int32_t *offsets);
+/* its gradients: dxs[r] = w[e]^T dys[r], and dw[e] = sum over e's rows of dys[r] xs[r]^T (accumulate, out_type: as in
+ * lookup_grad; an expert without rows has a block of zeros, or is left as it is). */
+int sparse_amd_tokens_experts_grad_x(struct futhark_context *ctx, void *stream, int type, void *dxs, int64_t ldx,
+                                     const void *dys, int64_t ldy, int64_t rows, const void *w, int64_t X, int64_t F,
+                                     int64_t D, int64_t ldw, int64_t blockw, const int32_t *offsets);
+int sparse_amd_tokens_experts_grad_w(struct futhark_context *ctx, void *stream, int type, int out_type, int accumulate,
+                                     void *dw, int64_t X, int64_t F, int64_t D, int64_t ldw, int64_t blockw,
+                                     const void *dys, int64_t ldy, const void *xs, int64_t ldx, int64_t rows,
+                                     const int32_t *offsets);
+
 /* ------------------------------------------------- (3) context extensions
  * No counterpart in the generated API. */
 /* Run all subsequent work on the caller's HIP stream (hipStream_t); the context

@@ -1,0 +1,562 @@
+// tokens.hip -- the sparse_amd_tokens_* entries of include/sparse_amd.h: argument checks, workspaces, launches.
+//
+// These entries take plain device pointers with row strides and the stream to run on.  They allocate nothing, keep
+// nothing from one call to the next and never wait, so they may be captured into a graph; the caller's device is the
+// current one again when they return.
+#include "tokens_rows.hpp"
+#include "tokens_lookup_grad.hpp"
+#include "tokens_experts.hpp"
+
+#include <initializer_list>
+
+using namespace samd;
+using namespace samd::tok;
+
+namespace {
+
+struct OnDevice {
+  std::lock_guard<std::mutex> g;
+  int before = -1;
+  explicit OnDevice(futhark_context *ctx) : g(ctx->mu) {
+    if (ctx->own_stream && hipGetDevice(&before) == hipSuccess && before != ctx->device) (void)hipSetDevice(ctx->device);
+    else before = -1;
+    ctx->n_entries++;
+  }
+  ~OnDevice() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+// A context whose device could not be opened launches nothing; arguments are checked all the same, before that is looked at.
+int need_device(futhark_context *ctx) {
+  return ctx->own_stream ? 0 : set_error(ctx, "context has no usable HIP device; libsparse_amd has no CPU path");
+}
+
+// Runs `body` with the context locked and its device current; no exception leaves.
+template <class F>
+int entry(futhark_context *ctx, F body) {
+  try {
+    OnDevice on(ctx);
+    return body();
+  } catch (...) {
+    return 1;
+  }
+}
+
+template <class T>
+struct Tag { typedef T type; };
+
+template <class F>
+int by_type(futhark_context *ctx, const char *who, int type, F f) {
+  switch (type) {
+    case SPARSE_AMD_F32: return f(Tag<float>());
+    case SPARSE_AMD_F16: return f(Tag<f16>());
+    case SPARSE_AMD_BF16: return f(Tag<bf16>());
+  }
+  return set_error(ctx, "%s: unknown element type %d", who, type);
+}
+
+template <class F>
+int by_type16(futhark_context *ctx, const char *who, int type, F f) {
+  switch (type) {
+    case SPARSE_AMD_F16: return f(Tag<f16>());
+    case SPARSE_AMD_BF16: return f(Tag<bf16>());
+    case SPARSE_AMD_F32: return set_error(ctx, "%s: the experts' products are offered for 16-bit elements", who);
+  }
+  return set_error(ctx, "%s: unknown element type %d", who, type);
+}
+
+template <class F>
+int by_index(futhark_context *ctx, const char *who, int bits, F f) {
+  if (bits == 32) return f(Tag<int32_t>());
+  if (bits == 64) return f(Tag<int64_t>());
+  return set_error(ctx, "%s: indices have 32 or 64 bits, not %d", who, bits);
+}
+
+int64_t type_size(int type) { return type == SPARSE_AMD_F32 ? 4 : 2; }
+
+// A panel of `rows` rows of `cols` elements of `size` bytes, `ld` elements apart; null where there is none.
+struct Panel {
+  const char *name;
+  const void *p;
+  int64_t rows, cols, ld, size;
+  int64_t bytes() const { return rows > 0 && cols > 0 ? ((rows - 1) * ld + cols) * size : 0; }
+};
+
+// Every panel has a place and a stride that keeps its rows apart; the results (the first `outs` panels) share no byte
+// with each other or with what is read.
+int check_panels(futhark_context *ctx, const char *who, int outs, std::initializer_list<Panel> panels) {
+  for (const Panel &a : panels) {
+    if (a.rows < 0 || a.cols < 0) return set_error(ctx, "%s: %s has a negative size", who, a.name);
+    if (a.rows > 1 && a.ld < a.cols) return set_error(ctx, "%s: the rows of %s are %lld apart and %lld long", who, a.name, (long long)a.ld, (long long)a.cols);
+    if (a.ld > ((int64_t)1 << 40) || a.rows > ((int64_t)1 << 40) || a.cols > ((int64_t)1 << 40) ||
+        (a.rows > 0 && a.ld > 0 && a.rows > ((int64_t)1 << 56) / a.ld))
+      return set_error(ctx, "%s: %s is too large", who, a.name);
+    if (a.bytes() > 0 && !a.p) return set_error(ctx, "%s: %s is null", who, a.name);
+    if (a.p && (uintptr_t)a.p % (uintptr_t)a.size) return set_error(ctx, "%s: %s is not aligned to its elements", who, a.name);
+  }
+  int i = 0;
+  for (const Panel *a = panels.begin(); a != panels.end() && i < outs; a++, i++)
+    for (const Panel *b = a + 1; b != panels.end(); b++) {
+      const char *pa = (const char *)a->p, *pb = (const char *)b->p;
+      if (a->bytes() > 0 && b->bytes() > 0 && pa < pb + b->bytes() && pb < pa + a->bytes())
+        return set_error(ctx, "%s: %s overlaps %s", who, a->name, b->name);
+    }
+  return 0;
+}
+
+int check_blocks(futhark_context *ctx, const char *who, int64_t blocks) {
+  if (blocks > 0x7fffffff) return set_error(ctx, "%s: more work than one launch can hold", who);
+  return 0;
+}
+
+#define TOK_LAUNCH(ctx, kernel, blocks, threads, stream, ...)                                                  \
+  do {                                                                                                         \
+    SAMD_TRY(need_device(ctx));                                                                                \
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks)), dim3((unsigned)(threads)), 0, stream, __VA_ARGS__);    \
+    SAMD_LAUNCH_CHECK(ctx);                                                                                    \
+  } while (0)
+
+// Rows in pieces of U = 4 keep four loads in flight per lane; a launch too small to fill the card with such waves is
+// spread over more of them instead.
+constexpr int64_t kFullCard = 2048;
+
+// ---------------------------------------------------------------- workspaces
+struct Carve {  // adds up 256-byte aligned parts of a workspace
+  char *base;
+  int64_t used = 0;
+  explicit Carve(void *p) : base((char *)p) {}
+  template <class T>
+  T *take(int64_t count) {
+    T *p = base ? (T *)(base + used) : nullptr;
+    used += (count * (int64_t)sizeof(T) + 255) & ~(int64_t)255;
+    return p;
+  }
+};
+
+struct Split {  // a split pass: its workgroups and how many items each has
+  int64_t per_group;
+  int groups;
+  explicit Split(int64_t n) {
+    per_group = cdiv(cdiv(n, kMaxGroups), kTile) * kTile;
+    groups = (int)cdiv(n, per_group);
+  }
+};
+
+struct GradPlan {
+  GradShape g;
+  bool small;
+  int passes, bits;
+  Split split;
+  uint32_t *keys, *keys2, *clear, *marks;
+  int32_t *items, *items2;
+  int *hist, *next_hist;
+  float *part;
+  int64_t clear_words, mark_words, bytes;
+
+  GradPlan(void *work, int type, int64_t n, int64_t V, int64_t D) : split(n > 0 ? n : 1) {
+    const int64_t per = 16 / type_size(type);
+    g.n = n; g.V = V; g.D = D;
+    g.segs = cdiv(cdiv(D, per), kWave);
+    // chunks of 32 read a key, an item and two chunk ends for 32 rows; where that leaves the card empty, chunks of 8
+    g.chunk = cdiv(n, 32) * g.segs >= kFullCard ? 32 : 8;
+    g.chunks = cdiv(n, g.chunk);
+    mark_words = cdiv(V, 32);
+    small = n <= kOneGroup && mark_words <= ((int64_t)1 << 17);
+    const int key_bits = bits_for(V + 1) > 0 ? bits_for(V + 1) : 1;
+    const int most = small ? kSmallBits : 10;
+    passes = (key_bits + most - 1) / most;
+    bits = (key_bits + passes - 1) / passes;
+    Carve c(work);
+    keys = c.take<uint32_t>(n);
+    items = c.take<int32_t>(n);
+    keys2 = nullptr; items2 = nullptr; hist = nullptr; next_hist = nullptr; clear = nullptr; clear_words = 0;
+    if (small) {
+      marks = c.take<uint32_t>(mark_words);
+    } else {
+      keys2 = c.take<uint32_t>(n);
+      items2 = c.take<int32_t>(n);
+      const int64_t counts = (int64_t)split.groups << bits;
+      hist = c.take<int>(counts);
+      clear_words = counts * (passes - 1) + mark_words;  // later passes' counts, then the marks
+      clear = c.take<uint32_t>(clear_words);
+      next_hist = (int *)clear;
+      marks = clear ? clear + counts * (passes - 1) : nullptr;
+    }
+    part = c.take<float>(g.chunks > 1 ? g.chunks * 2 * g.segs * kWave * per : 0);
+    bytes = c.used;
+  }
+};
+
+int check_work(futhark_context *ctx, const char *who, const void *work, int64_t have, int64_t need) {
+  if (need == 0) return 0;
+  if (!work || have < need) return set_error(ctx, "%s: needs a workspace of %lld bytes, got %lld", who, (long long)need, (long long)(work ? have : 0));
+  if ((uintptr_t)work % 256) return set_error(ctx, "%s: the workspace is not aligned to 256 bytes", who);
+  return 0;
+}
+
+template <class I>
+int order_ids(futhark_context *ctx, hipStream_t stream, const I *ids, const GradPlan &p, bool marked) {
+  uint32_t *marks = marked ? p.marks : nullptr;
+  const int n = (int)p.g.n;
+  if (p.small) {
+    if (n <= 1024)
+      TOK_LAUNCH(ctx, (id_sort_small_kernel<I, 1>), 1, 1024, stream, ids, n, p.g.V, p.passes, p.bits, p.keys, p.items, marks, p.mark_words);
+    else if (n <= 4096)
+      TOK_LAUNCH(ctx, (id_sort_small_kernel<I, 4>), 1, 1024, stream, ids, n, p.g.V, p.passes, p.bits, p.keys, p.items, marks, p.mark_words);
+    else
+      TOK_LAUNCH(ctx, (id_sort_small_kernel<I, 8>), 1, 1024, stream, ids, n, p.g.V, p.passes, p.bits, p.keys, p.items, marks, p.mark_words);
+    return 0;
+  }
+  const int bins = 1 << p.bits, mask = bins - 1;
+  const int64_t counts = (int64_t)p.split.groups << p.bits;
+  const Digits<1, I> d0 = {ids, nullptr, p.g.n, p.g.V, 0, mask};
+  TOK_LAUNCH(ctx, (digit_count_kernel<1, I>), p.split.groups, kThreads, stream, d0, p.split.per_group, bins, p.hist, p.clear, p.clear_words);
+  for (int k = 0; k < p.passes; k++) {
+    const bool last = k == p.passes - 1, to_first = (p.passes - 1 - k) % 2 == 0;
+    PassOut o = {};
+    o.keys = to_first ? p.keys : p.keys2;
+    o.items = to_first ? p.items : p.items2;
+    if (!last) {
+      o.next_hist = p.next_hist + counts * k;
+      o.next_shift = (k + 1) * p.bits;
+      o.next_mask = mask;
+      o.next_bins = bins;
+    }
+    if (k == 0) {
+      o.marks = marks;
+      TOK_LAUNCH(ctx, (digit_place_kernel<1, I>), p.split.groups, kThreads, stream, d0, p.split.per_group, bins, p.bits, (const int *)p.hist, o);
+    } else {
+      o.items_in = to_first ? p.items2 : p.items;
+      const Digits<2, I> d = {nullptr, to_first ? p.keys2 : p.keys, p.g.n, p.g.V, k * p.bits, mask};
+      TOK_LAUNCH(ctx, (digit_place_kernel<2, I>), p.split.groups, kThreads, stream, d, p.split.per_group, bins, p.bits,
+                 (const int *)(p.next_hist + counts * (k - 1)), o);
+    }
+  }
+  return 0;
+}
+
+template <class T, class TO, bool ADD>
+int sum_ids(futhark_context *ctx, hipStream_t stream, TO *dE, const T *dy, const float *vals, float scale, GradPlan &p) {
+  const int64_t fill_units = cdiv(p.g.D, kPer<TO>);
+  p.g.fill_segs = ADD ? 0 : cdiv(fill_units, kWave * kFillPieces);
+  const int64_t blocks = cdiv(p.g.chunks * p.g.segs + p.g.V * p.g.fill_segs, kWaves);
+  SAMD_TRY(check_blocks(ctx, "lookup_grad", blocks));
+  SAMD_TRY(check_blocks(ctx, "lookup_grad", p.g.chunks * p.g.segs));
+  TOK_LAUNCH(ctx, (lookup_grad_kernel<T, TO, ADD>), blocks, kThreads, stream, dE, dy, vals, scale, (const uint32_t *)p.keys,
+             (const int32_t *)p.items, (const uint32_t *)p.marks, p.part, p.g);
+  if (p.g.chunks > 1)
+    TOK_LAUNCH(ctx, (lookup_grad_join_kernel<T, TO, ADD>), p.g.chunks * p.g.segs, kThreads, stream, dE, (const uint32_t *)p.keys, p.part, p.g);
+  return 0;
+}
+
+// ---------------------------------------------------------------- experts
+template <class T>
+bool direct_to_lds(const T *p, int64_t ld) {
+  return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && ld <= ((int64_t)1 << 22);
+}
+
+template <class T, class TO, int KIND, int BM, int BN, int WM, int WN, bool FAST, bool ADD>
+int launch_experts(futhark_context *ctx, const char *who, hipStream_t stream, TO *C, const T *A, const T *B, const int32_t *offsets,
+                   ProductShape g) {
+  const int64_t n_tiles = cdiv(g.N, BN);
+  int64_t m_tiles, blocks;
+  if (KIND == kGradW) {
+    m_tiles = cdiv(g.M, BM);
+    blocks = g.X * m_tiles * n_tiles;
+  } else {
+    // every expert with rows ends in one tile that may not be full
+    m_tiles = g.rows / BM + (g.rows < g.X ? g.rows : g.X);
+    blocks = m_tiles * n_tiles;
+  }
+  SAMD_TRY(check_blocks(ctx, who, blocks));
+  g.m_tiles = (int)m_tiles;
+  g.n_tiles = (int)n_tiles;
+  TOK_LAUNCH(ctx, (experts_kernel<T, TO, KIND, BM, BN, WM, WN, FAST, ADD>), blocks, WM * WN * kWave, stream, C, A, B, offsets, g);
+  return 0;
+}
+
+template <class T, int KIND>
+int experts_panels(futhark_context *ctx, const char *who, hipStream_t stream, T *C, const T *A, const T *B, const int32_t *offsets,
+                   const ProductShape &g) {
+  const bool fast = direct_to_lds(A, g.ldA) && g.K % 8 == 0 && direct_to_lds(B, g.ldB) && g.blockB % 8 == 0;
+  if (!fast) return launch_experts<T, T, KIND, 128, 128, 2, 2, false, false>(ctx, who, stream, C, A, B, offsets, g);
+  const int64_t mean = g.rows / g.X;
+  if (mean <= 32) return launch_experts<T, T, KIND, 32, 128, 1, 4, true, false>(ctx, who, stream, C, A, B, offsets, g);
+  if (mean < 256) return launch_experts<T, T, KIND, 128, 128, 2, 2, true, false>(ctx, who, stream, C, A, B, offsets, g);
+  return launch_experts<T, T, KIND, 256, 256, 2, 4, true, false>(ctx, who, stream, C, A, B, offsets, g);
+}
+
+template <class T, class TO, bool ADD>
+int experts_weights(futhark_context *ctx, const char *who, hipStream_t stream, TO *C, const T *A, const T *B, const int32_t *offsets,
+                    const ProductShape &g) {
+  if (!(direct_to_lds(A, g.ldA) && direct_to_lds(B, g.ldB)))
+    return launch_experts<T, TO, kGradW, 128, 128, 2, 2, false, ADD>(ctx, who, stream, C, A, B, offsets, g);
+  return launch_experts<T, TO, kGradW, 128, 128, 2, 2, true, ADD>(ctx, who, stream, C, A, B, offsets, g);
+}
+
+int check_experts(futhark_context *ctx, const char *who, int64_t rows, int64_t X, int64_t F, int64_t D, const int32_t *offsets) {
+  if (rows < 0 || F < 0 || D < 0) return set_error(ctx, "%s: negative size", who);
+  if (X < 1 || X > kMaxExperts) return set_error(ctx, "%s: %lld experts (1 to %d are offered)", who, (long long)X, kMaxExperts);
+  if (rows > 0x7fffffff) return set_error(ctx, "%s: %lld rows (places have 31 bits)", who, (long long)rows);
+  if (F > 0x3fffffff || D > 0x3fffffff) return set_error(ctx, "%s: a block of %lld x %lld is too large", who, (long long)F, (long long)D);
+  if (!offsets) return set_error(ctx, "%s: offsets is null", who);
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sparse_amd_tokens_lookup(struct futhark_context *ctx, void *stream, int type, void *y, int64_t ldy, const void *table, int64_t V,
+                             int64_t D, int64_t ldt, const void *ids, int id_bits, int64_t n, const float *vals, float scale) {
+  return entry(ctx, [&]() -> int {
+    const char *who = "lookup";
+    return by_type(ctx, who, type, [&](auto t) {
+      return by_index(ctx, who, id_bits, [&](auto it) -> int {
+        typedef typename decltype(t)::type T;
+        typedef typename decltype(it)::type I;
+        SAMD_TRY(check_panels(ctx, who, 1, {{"the result", y, n, D, ldy, (int64_t)sizeof(T)}, {"the table", table, V, D, ldt, (int64_t)sizeof(T)},
+                                            {"ids", ids, 1, n, n, (int64_t)sizeof(I)}, {"vals", vals, 1, vals ? n : 0, n, 4}}));
+        if (n == 0 || D == 0) return 0;
+        const hipStream_t s = (hipStream_t)stream;
+        const int64_t units = cdiv(D, kPer<T>);
+        RowDeal d = deal_rows(n, units, 4);
+        const int u = d.lg == 6 && d.waves >= kFullCard ? 4 : 1;
+        if (u == 1) d = deal_rows(n, units, 1);
+        SAMD_TRY(check_blocks(ctx, who, cdiv(d.waves, kWaves)));
+        if (u == 4)
+          TOK_LAUNCH(ctx, (lookup_kernel<T, I, 4>), cdiv(d.waves, kWaves), kThreads, s, (T *)y, ldy, (const T *)table, ldt, V, D, (const I *)ids, n, vals, scale, d.lg, d.segs);
+        else
+          TOK_LAUNCH(ctx, (lookup_kernel<T, I, 1>), cdiv(d.waves, kWaves), kThreads, s, (T *)y, ldy, (const T *)table, ldt, V, D, (const I *)ids, n, vals, scale, d.lg, d.segs);
+        return 0;
+      });
+    });
+  });
+}
+
+int sparse_amd_tokens_lookup_dots(struct futhark_context *ctx, void *stream, int type, float *dvals, const void *dy, int64_t ldy,
+                                  const void *table, int64_t V, int64_t D, int64_t ldt, const void *ids, int id_bits, int64_t n,
+                                  float scale) {
+  return entry(ctx, [&]() -> int {
+    const char *who = "lookup_dots";
+    return by_type(ctx, who, type, [&](auto t) {
+      return by_index(ctx, who, id_bits, [&](auto it) -> int {
+        typedef typename decltype(t)::type T;
+        typedef typename decltype(it)::type I;
+        SAMD_TRY(check_panels(ctx, who, 1, {{"the result", dvals, 1, n, n, 4}, {"dy", dy, n, D, ldy, (int64_t)sizeof(T)},
+                                            {"the table", table, V, D, ldt, (int64_t)sizeof(T)}, {"ids", ids, 1, n, n, (int64_t)sizeof(I)}}));
+        if (n == 0) return 0;
+        SAMD_TRY(check_blocks(ctx, who, cdiv(n, kWaves)));
+        TOK_LAUNCH(ctx, (lookup_dots_kernel<T, I>), cdiv(n, kWaves), kThreads, (hipStream_t)stream, dvals, (const T *)dy, ldy, (const T *)table, ldt, V, D, (const I *)ids, n, scale);
+        return 0;
+      });
+    });
+  });
+}
+
+int64_t sparse_amd_tokens_lookup_grad_workspace(int type, int64_t n, int64_t V, int64_t D) {
+  if (n <= 0 || V < 0 || D <= 0) return 0;
+  return GradPlan(nullptr, type, n, V, D).bytes;
+}
+
+int sparse_amd_tokens_lookup_grad(struct futhark_context *ctx, void *stream, int type, int out_type, int accumulate, void *dtable,
+                                  int64_t V, int64_t D, int64_t ldt, const void *dy, int64_t ldy, const void *ids, int id_bits, int64_t n,
+                                  const float *vals, float scale, void *work, int64_t work_bytes) {
+  return entry(ctx, [&]() -> int {
+    const char *who = "lookup_grad";
+    if (out_type != type && out_type != SPARSE_AMD_F32)
+      return set_error(ctx, "%s: the gradient has the rows' element type or 32 bits", who);
+    if (V > 0x7ffffffe || n > 0x7fffffff) return set_error(ctx, "%s: rows and ids are counted in 31 bits", who);
+    return by_type(ctx, who, type, [&](auto t) {
+      return by_index(ctx, who, id_bits, [&](auto it) -> int {
+        typedef typename decltype(t)::type T;
+        typedef typename decltype(it)::type I;
+        SAMD_TRY(check_panels(ctx, who, 1, {{"the result", dtable, V, D, ldt, type_size(out_type)}, {"dy", dy, n, D, ldy, (int64_t)sizeof(T)},
+                                            {"ids", ids, 1, n, n, (int64_t)sizeof(I)}, {"vals", vals, 1, vals ? n : 0, n, 4},
+                                            {"the workspace", work, 1, work ? work_bytes : 0, work_bytes, 1}}));
+        if (V == 0 || D == 0 || (n == 0 && accumulate)) return 0;
+        const hipStream_t s = (hipStream_t)stream;
+        GradPlan p(n > 0 ? work : nullptr, type, n, V, D);
+        if (n > 0) SAMD_TRY(check_work(ctx, who, work, work_bytes, p.bytes));
+        p.g.ldy = ldy;
+        p.g.ldE = ldt;
+        if (n > 0) SAMD_TRY(order_ids<I>(ctx, s, (const I *)ids, p, !accumulate));  // without ids there are no marks: all rows are zeroed
+        if (out_type == type)
+          return accumulate ? sum_ids<T, T, true>(ctx, s, (T *)dtable, (const T *)dy, vals, scale, p)
+                            : sum_ids<T, T, false>(ctx, s, (T *)dtable, (const T *)dy, vals, scale, p);
+        return accumulate ? sum_ids<T, float, true>(ctx, s, (float *)dtable, (const T *)dy, vals, scale, p)
+                          : sum_ids<T, float, false>(ctx, s, (float *)dtable, (const T *)dy, vals, scale, p);
+      });
+    });
+  });
+}
+
+int64_t sparse_amd_tokens_route_workspace(int64_t n, int64_t X) {
+  if (n <= kOneGroup || X < 1) return 0;
+  return (Split(n).groups * (X + 1) * (int64_t)sizeof(int) + 255) & ~(int64_t)255;
+}
+
+int sparse_amd_tokens_route(struct futhark_context *ctx, void *stream, const void *chosen, int id_bits, int64_t n, int64_t X, int32_t *pos,
+                            int32_t *src, int32_t *offsets, void *work, int64_t work_bytes) {
+  return entry(ctx, [&]() -> int {
+    const char *who = "route";
+    if (X < 1 || X > kMaxExperts) return set_error(ctx, "%s: %lld experts (1 to %d are offered)", who, (long long)X, kMaxExperts);
+    if (n > 0x7fffffff) return set_error(ctx, "%s: %lld choices (places have 31 bits)", who, (long long)n);
+    return by_index(ctx, who, id_bits, [&](auto it) -> int {
+      typedef typename decltype(it)::type I;
+      SAMD_TRY(check_panels(ctx, who, 3, {{"pos", pos, 1, n, n, 4}, {"src", src, 1, n, n, 4}, {"offsets", offsets, 1, X + 1, X + 1, 4},
+                                          {"chosen", chosen, 1, n, n, (int64_t)sizeof(I)}, {"the workspace", work, 1, work ? work_bytes : 0, work_bytes, 1}}));
+      const hipStream_t s = (hipStream_t)stream;
+      const int bits = bits_for(X + 1);
+      if (n <= 256)
+        TOK_LAUNCH(ctx, (route_small_kernel<I, 4, 1>), 1, 256, s, (const I *)chosen, (int)n, (int)X, bits, pos, src, offsets);
+      else if (n <= 1024)
+        TOK_LAUNCH(ctx, (route_small_kernel<I, 16, 1>), 1, 1024, s, (const I *)chosen, (int)n, (int)X, bits, pos, src, offsets);
+      else if (n <= kOneGroup)
+        TOK_LAUNCH(ctx, (route_small_kernel<I, 16, 8>), 1, 1024, s, (const I *)chosen, (int)n, (int)X, bits, pos, src, offsets);
+      else {
+        SAMD_TRY(check_work(ctx, who, work, work_bytes, sparse_amd_tokens_route_workspace(n, X)));
+        const Split sp(n);
+        const Digits<0, I> d = {(const I *)chosen, nullptr, n, X, 0, 0};
+        TOK_LAUNCH(ctx, (digit_count_kernel<0, I>), sp.groups, kThreads, s, d, sp.per_group, (int)X + 1, (int *)work, (uint32_t *)nullptr, (int64_t)0);
+        PassOut o = {};
+        o.pos = pos; o.src = src; o.offsets = offsets;
+        TOK_LAUNCH(ctx, (digit_place_kernel<0, I>), sp.groups, kThreads, s, d, sp.per_group, (int)X + 1, bits, (const int *)work, o);
+      }
+      return 0;
+    });
+  });
+}
+
+int sparse_amd_tokens_dispatch(struct futhark_context *ctx, void *stream, int type, void *xs, int64_t ldxs, int64_t slots, const void *x,
+                               int64_t ldx, int64_t n, int64_t D, int64_t K, const int32_t *pos, const float *weights) {
+  return entry(ctx, [&]() -> int {
+    const char *who = "dispatch";
+    if (K < 0 || K > 0x7fffffff) return set_error(ctx, "%s: %lld places a row", who, (long long)K);
+    return by_type(ctx, who, type, [&](auto t) -> int {
+      typedef typename decltype(t)::type T;
+      SAMD_TRY(check_panels(ctx, who, 1, {{"the result", xs, slots, D, ldxs, (int64_t)sizeof(T)}, {"x", x, n, D, ldx, (int64_t)sizeof(T)},
+                                          {"pos", pos, n, K, K, 4}, {"weights", weights, weights ? n : 0, K, K, 4}}));
+      if (n == 0 || D == 0 || K == 0) return 0;
+      const hipStream_t s = (hipStream_t)stream;
+      const int64_t units = cdiv(D, kPer<T>);
+      RowDeal d = deal_rows(n, units, 4);
+      const int u = d.lg == 6 && d.waves >= kFullCard ? 4 : 1;
+      if (u == 1) d = deal_rows(n, units, 1);
+      SAMD_TRY(check_blocks(ctx, who, cdiv(d.waves, kWaves)));
+      if (u == 4)
+        TOK_LAUNCH(ctx, (dispatch_kernel<T, 4>), cdiv(d.waves, kWaves), kThreads, s, (T *)xs, ldxs, (const T *)x, ldx, n, D, (int)K, pos, slots, weights, d.lg, d.segs);
+      else
+        TOK_LAUNCH(ctx, (dispatch_kernel<T, 1>), cdiv(d.waves, kWaves), kThreads, s, (T *)xs, ldxs, (const T *)x, ldx, n, D, (int)K, pos, slots, weights, d.lg, d.segs);
+      return 0;
+    });
+  });
+}
+
+int sparse_amd_tokens_combine(struct futhark_context *ctx, void *stream, int type, void *y, int64_t ldy, const void *ys, int64_t ldys,
+                              int64_t slots, int64_t n, int64_t D, int64_t K, const int32_t *pos, const float *weights) {
+  return entry(ctx, [&]() -> int {
+    const char *who = "combine";
+    if (K < 0 || K > 0x7fffffff) return set_error(ctx, "%s: %lld places a row", who, (long long)K);
+    return by_type(ctx, who, type, [&](auto t) -> int {
+      typedef typename decltype(t)::type T;
+      SAMD_TRY(check_panels(ctx, who, 1, {{"the result", y, n, D, ldy, (int64_t)sizeof(T)}, {"ys", ys, slots, D, ldys, (int64_t)sizeof(T)},
+                                          {"pos", pos, n, K, K, 4}, {"weights", weights, weights ? n : 0, K, K, 4}}));
+      if (n == 0 || D == 0) return 0;
+      const hipStream_t s = (hipStream_t)stream;
+      const RowDeal d = deal_rows(n, cdiv(D, kPer<T>), 1);
+      SAMD_TRY(check_blocks(ctx, who, cdiv(d.waves, kWaves)));
+      TOK_LAUNCH(ctx, (combine_kernel<T, 1>), cdiv(d.waves, kWaves), kThreads, s, (T *)y, ldy, (const T *)ys, ldys, n, D, (int)K, pos, slots, weights, d.lg, d.segs);
+      return 0;
+    });
+  });
+}
+
+int sparse_amd_tokens_combine_grad(struct futhark_context *ctx, void *stream, int type, void *dys, int64_t lddys, float *dweights,
+                                   const void *dy, int64_t lddy, const void *ys, int64_t ldys, int64_t slots, int64_t n, int64_t D,
+                                   int64_t K, const int32_t *pos, const float *weights) {
+  return entry(ctx, [&]() -> int {
+    const char *who = "combine_grad";
+    if (K < 0 || K > 0x7fffffff) return set_error(ctx, "%s: %lld places a row", who, (long long)K);
+    return by_type(ctx, who, type, [&](auto t) -> int {
+      typedef typename decltype(t)::type T;
+      SAMD_TRY(check_panels(ctx, who, 2, {{"dys", dys, slots, D, lddys, (int64_t)sizeof(T)}, {"dweights", dweights, n, K, K, 4},
+                                          {"dy", dy, n, D, lddy, (int64_t)sizeof(T)}, {"ys", ys, slots, D, ldys, (int64_t)sizeof(T)},
+                                          {"pos", pos, n, K, K, 4}, {"weights", weights, n, K, K, 4}}));
+      if (n == 0 || K == 0) return 0;
+      SAMD_TRY(check_blocks(ctx, who, n));
+      TOK_LAUNCH(ctx, (combine_grad_kernel<T>), n, kThreads, (hipStream_t)stream, (T *)dys, lddys, dweights, (const T *)dy, lddy, (const T *)ys, ldys, D, (int)K, pos, slots, weights);
+      return 0;
+    });
+  });
+}
+
+int sparse_amd_tokens_experts(struct futhark_context *ctx, void *stream, int type, void *ys, int64_t ldy, const void *xs, int64_t ldx,
+                              int64_t rows, const void *w, int64_t X, int64_t F, int64_t D, int64_t ldw, int64_t blockw,
+                              const int32_t *offsets) {
+  return entry(ctx, [&]() -> int {
+    const char *who = "experts";
+    SAMD_TRY(check_experts(ctx, who, rows, X, F, D, offsets));
+    return by_type16(ctx, who, type, [&](auto t) -> int {
+      typedef typename decltype(t)::type T;
+      if (X > 1 && blockw < (F > 0 ? (F - 1) * ldw + D : 0)) return set_error(ctx, "%s: the blocks of w overlap", who);
+      SAMD_TRY(check_panels(ctx, who, 1, {{"the result", ys, rows, F, ldy, 2}, {"xs", xs, rows, D, ldx, 2},
+                                          {"w", w, X, F > 0 ? (F - 1) * ldw + D : 0, X > 1 ? blockw : (F - 1) * ldw + D, 2}, {"a block of w", w, F, D, ldw, 2},
+                                          {"offsets", offsets, 1, X + 1, X + 1, 4}}));
+      if (rows == 0 || F == 0) return 0;
+      ProductShape g = {};
+      g.rows = rows; g.N = F; g.K = D; g.ldA = ldx; g.ldB = ldw; g.ldC = ldy; g.blockB = blockw; g.X = (int)X;
+      return experts_panels<T, kForward>(ctx, who, (hipStream_t)stream, (T *)ys, (const T *)xs, (const T *)w, offsets, g);
+    });
+  });
+}
+
+int sparse_amd_tokens_experts_grad_x(struct futhark_context *ctx, void *stream, int type, void *dxs, int64_t ldx, const void *dys,
+                                     int64_t ldy, int64_t rows, const void *w, int64_t X, int64_t F, int64_t D, int64_t ldw,
+                                     int64_t blockw, const int32_t *offsets) {
+  return entry(ctx, [&]() -> int {
+    const char *who = "experts_grad_x";
+    SAMD_TRY(check_experts(ctx, who, rows, X, F, D, offsets));
+    return by_type16(ctx, who, type, [&](auto t) -> int {
+      typedef typename decltype(t)::type T;
+      if (X > 1 && blockw < (F > 0 ? (F - 1) * ldw + D : 0)) return set_error(ctx, "%s: the blocks of w overlap", who);
+      SAMD_TRY(check_panels(ctx, who, 1, {{"the result", dxs, rows, D, ldx, 2}, {"dys", dys, rows, F, ldy, 2},
+                                          {"w", w, X, F > 0 ? (F - 1) * ldw + D : 0, X > 1 ? blockw : (F - 1) * ldw + D, 2}, {"a block of w", w, F, D, ldw, 2},
+                                          {"offsets", offsets, 1, X + 1, X + 1, 4}}));
+      if (rows == 0 || D == 0) return 0;
+      ProductShape g = {};
+      g.rows = rows; g.N = D; g.K = F; g.ldA = ldy; g.ldB = ldw; g.ldC = ldx; g.blockB = blockw; g.X = (int)X;
+      return experts_panels<T, kGradX>(ctx, who, (hipStream_t)stream, (T *)dxs, (const T *)dys, (const T *)w, offsets, g);
+    });
+  });
+}
+
+int sparse_amd_tokens_experts_grad_w(struct futhark_context *ctx, void *stream, int type, int out_type, int accumulate, void *dw,
+                                     int64_t X, int64_t F, int64_t D, int64_t ldw, int64_t blockw, const void *dys, int64_t ldy,
+                                     const void *xs, int64_t ldx, int64_t rows, const int32_t *offsets) {
+  return entry(ctx, [&]() -> int {
+    const char *who = "experts_grad_w";
+    SAMD_TRY(check_experts(ctx, who, rows, X, F, D, offsets));
+    if (out_type != type && out_type != SPARSE_AMD_F32)
+      return set_error(ctx, "%s: the gradient has the rows' element type or 32 bits", who);
+    return by_type16(ctx, who, type, [&](auto t) -> int {
+      typedef typename decltype(t)::type T;
+      if (X > 1 && blockw < (F > 0 ? (F - 1) * ldw + D : 0)) return set_error(ctx, "%s: the blocks of dw overlap", who);
+      SAMD_TRY(check_panels(ctx, who, 1, {{"the result", dw, X, F > 0 ? (F - 1) * ldw + D : 0, X > 1 ? blockw : (F - 1) * ldw + D, type_size(out_type)},
+                                          {"dys", dys, rows, F, ldy, 2}, {"xs", xs, rows, D, ldx, 2}, {"offsets", offsets, 1, X + 1, X + 1, 4}}));
+      SAMD_TRY(check_panels(ctx, who, 0, {{"a block of the result", dw, F, D, ldw, type_size(out_type)}}));
+      if (F == 0 || D == 0) return 0;
+      ProductShape g = {};
+      g.rows = rows; g.M = F; g.N = D; g.ldA = ldy; g.ldB = ldx; g.ldC = ldw; g.blockC = blockw; g.X = (int)X;
+      const hipStream_t s = (hipStream_t)stream;
+      if (out_type == type)
+        return accumulate ? experts_weights<T, T, true>(ctx, who, s, (T *)dw, (const T *)dys, (const T *)xs, offsets, g)
+                          : experts_weights<T, T, false>(ctx, who, s, (T *)dw, (const T *)dys, (const T *)xs, offsets, g);
+      return accumulate ? experts_weights<T, float, true>(ctx, who, s, (float *)dw, (const T *)dys, (const T *)xs, offsets, g)
+                        : experts_weights<T, float, false>(ctx, who, s, (float *)dw, (const T *)dys, (const T *)xs, offsets, g);
+    });
+  });
+}
+
+}  // extern "C"

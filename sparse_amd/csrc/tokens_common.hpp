@@ -1,0 +1,114 @@
+// tokens_common.hpp -- what the kernels of tokens.hip share: element types, 16-byte pieces of a row, wave sums.
+//
+// Everything here works on rows of a dense row-major panel: `units` pieces of 16 bytes, the last one possibly short.
+// Rows need no more alignment than their element: the hardware takes 128-bit global accesses at any element's address
+// (a piece that crosses a cache line costs a second line), so odd widths and strides run the same kernels as round ones.
+#pragma once
+
+#include "common.hpp"
+
+namespace samd {
+namespace tok {
+
+using bf16 = __bf16;
+using f16 = _Float16;
+
+constexpr int kWave = 64;
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+
+template <class T>
+constexpr int kPer = 16 / (int)sizeof(T);  // elements of a 16-byte piece
+
+template <class T>
+struct Piece {
+  T v[kPer<T>];
+};
+
+// The `left` elements (kPer or fewer) of a piece at p; what is not there reads as zero.
+template <class T>
+__device__ __forceinline__ Piece<T> load_piece(const T *p, int64_t left) {
+  Piece<T> r;
+  if (left >= kPer<T>) {
+    __builtin_memcpy(&r, p, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer<T>; i++) r.v[i] = i < left ? p[i] : (T)0.0f;
+  }
+  return r;
+}
+
+template <class T>
+__device__ __forceinline__ void store_piece(T *p, const Piece<T> &r, int64_t left) {
+  if (left >= kPer<T>) {
+    __builtin_memcpy(p, &r, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer<T>; i++)
+      if (i < left) p[i] = r.v[i];
+  }
+}
+
+// kPer<T> sums held in 32 bits, rounded once to TO (16 or 32 bits) and stored; ADD: added to what is there first.
+template <class T, class TO, bool ADD>
+__device__ __forceinline__ void store_sums(TO *p, const float (&s)[kPer<T>], int64_t left) {
+  if (left >= kPer<T>) {
+    TO o[kPer<T>];
+    if (ADD) __builtin_memcpy(o, p, sizeof o);
+#pragma unroll
+    for (int i = 0; i < kPer<T>; i++) o[i] = (TO)(ADD ? (float)o[i] + s[i] : s[i]);
+    __builtin_memcpy(p, o, sizeof o);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer<T>; i++)
+      if (i < left) p[i] = (TO)(ADD ? (float)p[i] + s[i] : s[i]);
+  }
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int d = kWave / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, kWave);
+  return v;
+}
+
+__device__ __forceinline__ int lane_id() { return (int)(threadIdx.x & (kWave - 1)); }
+// The same in every lane of a wave, and known to be: what is indexed by it is loaded once per wave.
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave)); }
+
+// How a launch deals rows to waves.  Rows of 64 pieces or more: a wave takes `u` x 64 pieces of one row, `segs` waves a
+// row.  Shorter rows: a power of two of lanes each (1 << lg), so that a wave takes several.
+struct RowDeal {
+  int lg;
+  int64_t segs;
+  int64_t waves;
+};
+
+inline RowDeal deal_rows(int64_t rows, int64_t units, int u) {
+  RowDeal d;
+  d.lg = 0;
+  while (d.lg < 6 && ((int64_t)1 << d.lg) < units) d.lg++;
+  d.segs = d.lg == 6 ? cdiv(units, (int64_t)kWave * u) : 1;
+  d.waves = cdiv(rows, (int64_t)(kWave >> d.lg)) * d.segs;
+  return d;
+}
+
+struct RowPlace {
+  int64_t row, unit;  // this lane's row, and its first piece in it
+};
+
+__device__ __forceinline__ RowPlace my_row(int lg, int64_t segs, int u) {
+  const int64_t w = (int64_t)blockIdx.x * kWaves + wave_id();
+  const int lane = lane_id();
+  RowPlace r;
+  if (lg == 6) {
+    r.row = w / segs;
+    r.unit = (w - r.row * segs) * (kWave * u) + lane;
+  } else {
+    r.row = w * (kWave >> lg) + (lane >> lg);
+    r.unit = lane & ((1 << lg) - 1);
+  }
+  return r;
+}
+
+}  // namespace tok
+}  // namespace samd
