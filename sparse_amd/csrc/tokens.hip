@@ -253,26 +253,30 @@ int sum_ids(futhark_context *ctx, hipStream_t stream, TO *dE, const T *dy, const
 // ---------------------------------------------------------------- experts
 template <class T>
 bool direct_to_lds(const T *p, int64_t ld) {
-  return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && ld <= ((int64_t)1 << 22);
+  return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && ld <= ((int64_t)1 << 20);
 }
 
-template <class T, class TO, int KIND, int BM, int BN, int WM, int WN, bool FAST, bool ADD>
+template <class T, class TO, int KIND, int BM, int BN, int DEPTH, int WM, int WN, bool ADD>
 int launch_experts(futhark_context *ctx, const char *who, hipStream_t stream, TO *C, const T *A, const T *B, const int32_t *offsets,
                    ProductShape g) {
   const int64_t n_tiles = cdiv(g.N, BN);
   int64_t m_tiles, blocks;
   if (KIND == kGradW) {
     m_tiles = cdiv(g.M, BM);
-    blocks = g.X * m_tiles * n_tiles;
+    blocks = g.X * (cdiv(m_tiles * n_tiles, kXcds) * kXcds);
   } else {
     // every expert with rows ends in one tile that may not be full
     m_tiles = g.rows / BM + (g.rows < g.X ? g.rows : g.X);
     blocks = m_tiles * n_tiles;
   }
+  blocks = cdiv(blocks, kXcds) * kXcds;
   SAMD_TRY(check_blocks(ctx, who, blocks));
   g.m_tiles = (int)m_tiles;
   g.n_tiles = (int)n_tiles;
-  TOK_LAUNCH(ctx, (experts_kernel<T, TO, KIND, BM, BN, WM, WN, FAST, ADD>), blocks, WM * WN * kWave, stream, C, A, B, offsets, g);
+  if constexpr (DEPTH == 0)
+    TOK_LAUNCH(ctx, (experts_any_kernel<T, TO, KIND, BM, BN, WM, WN, ADD>), blocks, WM * WN * kWave, stream, C, A, B, offsets, g);
+  else
+    TOK_LAUNCH(ctx, (experts_kernel<T, TO, KIND, BM, BN, DEPTH, WM, WN, ADD>), blocks, WM * WN * kWave, stream, C, A, B, offsets, g);
   return 0;
 }
 
@@ -280,19 +284,19 @@ template <class T, int KIND>
 int experts_panels(futhark_context *ctx, const char *who, hipStream_t stream, T *C, const T *A, const T *B, const int32_t *offsets,
                    const ProductShape &g) {
   const bool fast = direct_to_lds(A, g.ldA) && g.K % 8 == 0 && direct_to_lds(B, g.ldB) && g.blockB % 8 == 0;
-  if (!fast) return launch_experts<T, T, KIND, 128, 128, 2, 2, false, false>(ctx, who, stream, C, A, B, offsets, g);
+  if (!fast) return launch_experts<T, T, KIND, 128, 128, 0, 2, 2, false>(ctx, who, stream, C, A, B, offsets, g);
   const int64_t mean = g.rows / g.X;
-  if (mean <= 32) return launch_experts<T, T, KIND, 32, 128, 1, 4, true, false>(ctx, who, stream, C, A, B, offsets, g);
-  if (mean < 256) return launch_experts<T, T, KIND, 128, 128, 2, 2, true, false>(ctx, who, stream, C, A, B, offsets, g);
-  return launch_experts<T, T, KIND, 256, 256, 2, 4, true, false>(ctx, who, stream, C, A, B, offsets, g);
+  if (mean <= 32) return launch_experts<T, T, KIND, 32, 128, 64, 1, 4, false>(ctx, who, stream, C, A, B, offsets, g);
+  if (mean < 256) return launch_experts<T, T, KIND, 128, 128, 32, 2, 2, false>(ctx, who, stream, C, A, B, offsets, g);
+  return launch_experts<T, T, KIND, 256, 256, 32, 2, 4, false>(ctx, who, stream, C, A, B, offsets, g);
 }
 
 template <class T, class TO, bool ADD>
 int experts_weights(futhark_context *ctx, const char *who, hipStream_t stream, TO *C, const T *A, const T *B, const int32_t *offsets,
                     const ProductShape &g) {
   if (!(direct_to_lds(A, g.ldA) && direct_to_lds(B, g.ldB)))
-    return launch_experts<T, TO, kGradW, 128, 128, 2, 2, false, ADD>(ctx, who, stream, C, A, B, offsets, g);
-  return launch_experts<T, TO, kGradW, 128, 128, 2, 2, true, ADD>(ctx, who, stream, C, A, B, offsets, g);
+    return launch_experts<T, TO, kGradW, 128, 128, 0, 2, 2, ADD>(ctx, who, stream, C, A, B, offsets, g);
+  return launch_experts<T, TO, kGradW, 256, 256, 32, 2, 4, ADD>(ctx, who, stream, C, A, B, offsets, g);
 }
 
 int check_experts(futhark_context *ctx, const char *who, int64_t rows, int64_t X, int64_t F, int64_t D, const int32_t *offsets) {

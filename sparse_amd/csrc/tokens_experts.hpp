@@ -25,8 +25,6 @@ namespace tok {
 
 enum { kForward = 0, kGradX = 1, kGradW = 2 };
 
-constexpr int kDepth = 64;  // of the summed index in a step
-
 template <class T>
 struct Mfma;
 template <>
@@ -57,17 +55,25 @@ struct ProductShape {
   int m_tiles, n_tiles;  // kForward / kGradX: m_tiles = upper bound over all experts; kGradW: of one block
 };
 
-// One operand's tile: R rows of the result's index, kDepth of the summed index.
+// A value that every lane has, known to be the same: what is computed from it stays in scalar registers (a descriptor that
+// might differ between lanes would be loaded through lane by lane).
+__device__ __forceinline__ int64_t same(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
+// One operand's tile: R rows of the result's index, DEPTH (32 or 64) of the summed index.
 // p: element (0, 0) of the tile's first step; `rest`: elements from p to behind the operand's last one.
-template <class T, int R, bool STANDING, int NT, bool FAST>
+template <class T, int R, int DEPTH, bool STANDING, int NT, bool FAST>
 struct Tile {
-  static constexpr int kLoads = R * kDepth * (int)sizeof(T) / 16 / NT;  // 16-byte chunks a thread brings per step
-  static_assert(kLoads >= 1 && R * kDepth * (int)sizeof(T) / 16 % NT == 0, "a tile is a whole number of loads for every thread");
+  static constexpr int kLoads = R * DEPTH * (int)sizeof(T) / 16 / NT;  // 16-byte chunks a thread brings per step
+  static_assert(kLoads >= 1 && R * DEPTH * (int)sizeof(T) / 16 % NT == 0, "a tile is a whole number of loads for every thread");
 
   const T *p;
   int64_t ld, rest, summed;
   int64_t width;        // how much of the result's index there is from the tile's first on
   uint32_t off[FAST ? kLoads : 1];
+  __amdgpu_buffer_rsrc_t bounds;
   Piece<T> held[FAST ? 1 : kLoads];
 
   // the chunk that thread t's load i puts at LDS bytes (i * NT + t) * 16: its row in memory and its first column there
@@ -79,51 +85,71 @@ struct Tile {
       *row = k;
       *col = (((q >> 1) ^ spread(k)) << 4) + ((q & 1) << 3);
     } else {
-      const int r = at >> 3, q = at & 7;
+      constexpr int per = DEPTH / 8;
+      const int r = at / per, q = at % per;
       *row = r;
-      *col = (q ^ (r & 7)) << 3;
+      *col = (q ^ twist(r)) << 3;
     }
   }
+  // ds_read_b128 serves 16 lanes at a time, over 64 banks: lanes 0-3, 12-15 and 20-27, then 4-11, 16-19 and 28-31, and the
+  // same of the upper half.  Either set has to find its rows' chunks in 16 different places.
+  static __device__ __forceinline__ int twist(int r) { return DEPTH == 64 ? (r >> 1) & 7 : (4 - (r >> 2)) & 3; }
   static __device__ __forceinline__ int spread(int k) { return (k & 3) | (((k >> 3) & 1) << 2); }
 
   __device__ __forceinline__ void init(const T *base, int64_t ld_, int64_t rest_, int64_t summed_, int64_t width_) {
-    p = base; ld = ld_; rest = rest_; summed = summed_; width = width_;
-    if (FAST)
+    p = (const T *)same(reinterpret_cast<int64_t>(base)); ld = ld_; rest = same(rest_); summed = summed_; width = width_;
+    if (FAST) {
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
         int r, c;
         source(i, threadIdx.x, &r, &c);
         off[i] = (uint32_t)(((int64_t)r * ld + c) * (int64_t)sizeof(T));
       }
+      bound();
+    }
   }
 
-  // Starts bringing the step at summed index k0 into lds (FAST), or into registers.
-  __device__ __forceinline__ void bring(T *lds, int64_t k0) {
+  __device__ __forceinline__ void bound() {
+    const int64_t bytes = rest * (int64_t)sizeof(T);
+    bounds = __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, (int)(bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : bytes), 0x00020000);
+  }
+
+  // FAST: steps are counted from here on `steps` further, so that their offsets stay small whatever the operand's size.
+  __device__ __forceinline__ void move(int steps) {
+    const int64_t by = steps * DEPTH * (STANDING ? ld : 1);
+    p += by;
+    rest -= by;
+    summed -= steps * DEPTH;
+    bound();
+  }
+
+  // FAST: starts the loads of step `step` into lds.
+  __device__ __forceinline__ void start(T *lds, int step) {
+    int row, col;
+    source(0, threadIdx.x, &row, &col);  // the same columns in every load of a thread: NT / (DEPTH / 8) rows on, twist() repeats
+    // lying: columns beyond the summed index are the next row's, and are not read
+    const bool dead = !STANDING && col >= summed - step * DEPTH;
+    const int at = (int)(step * DEPTH * (STANDING ? ld : 1) * (int64_t)sizeof(T));
+    char *to = (char *)lds + wave_id() * (kWave * 16);
+#pragma unroll
+    for (int i = 0; i < kLoads; i++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(bounds, (LdsVoid *)(to + i * NT * 16), 16, (int)(dead ? 0x80000000u : off[i]), at, 0, 0);
+  }
+
+  // Not FAST: the step at summed index k0 into registers, and from there into lds.
+  __device__ __forceinline__ void bring(int64_t k0) {
     const int64_t step = STANDING ? k0 * ld : k0;
-    if (FAST) {
-      int64_t bytes = (rest - step) * (int64_t)sizeof(T);
-      bytes = bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : bytes;
-      const __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void *)(p + step), 0, (int)bytes, 0x00020000);
-      // lying: columns beyond the summed index are the next row's, and are not read
-      const bool dead = !STANDING && (((int)(threadIdx.x & 7) ^ (int)((threadIdx.x >> 3) & 7)) << 3) >= summed - k0;
-      char *to = (char *)lds + wave_id() * (kWave * 16);
 #pragma unroll
-      for (int i = 0; i < kLoads; i++)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (LdsVoid *)(to + i * NT * 16), 16, (int)(dead ? 0x80000000u : off[i]), 0, 0, 0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kLoads; i++) {
-        int r, c;
-        source(i, threadIdx.x, &r, &c);
-        const int64_t left = STANDING ? (k0 + r < summed ? width - c : 0) : (r < width ? summed - k0 - c : 0);
-        held[i] = load_piece(p + step + r * ld + c, left);
-      }
+    for (int i = 0; i < kLoads; i++) {
+      int r, c;
+      source(i, threadIdx.x, &r, &c);
+      const int64_t left = STANDING ? (k0 + r < summed ? width - c : 0) : (r < width ? summed - k0 - c : 0);
+      held[FAST ? 0 : i] = load_piece(p + step + r * ld + c, left);
     }
   }
   __device__ __forceinline__ void put(T *lds) {
-    if (!FAST)
 #pragma unroll
-      for (int i = 0; i < kLoads; i++) __builtin_memcpy((char *)lds + (i * NT + (int)threadIdx.x) * 16, &held[i], 16);
+    for (int i = 0; i < kLoads; i++) __builtin_memcpy((char *)lds + (i * NT + (int)threadIdx.x) * 16, &held[FAST ? 0 : i], 16);
   }
 
   // Fragment of rows r0 .. r0+15 and summed index 32 kk .. 32 kk + 31: lane l has row r0 + l % 16, eight k from 8 (l / 16) on.
@@ -140,7 +166,7 @@ struct Tile {
       __builtin_memcpy((char *)&f + 8, &b, 8);
     } else {
       const int r = r0 + (l & 15);
-      const T *at = lds + r * kDepth + (((kk * 4 + (l >> 4)) ^ (r & 7)) << 3);
+      const T *at = lds + r * DEPTH + (((kk * 4 + (l >> 4)) ^ twist(r)) << 3);
       f = *(const typename Mfma<T>::Frag *)at;
     }
     return f;
@@ -150,6 +176,34 @@ struct Tile {
 __device__ __forceinline__ int64_t clamped(const int32_t *offsets, int e, int64_t rows) {
   const int64_t v = offsets[e];
   return v < 0 ? 0 : v > rows ? rows : v;
+}
+
+constexpr int kXcds = 8;  // workgroup i runs on die i % 8, each with an L2 of its own
+
+// Tile `id` of m x n: every die has a run of neighbouring tiles, taken down columns of kDown tiles, so that the 32 tiles a
+// die works on at a time share 8 tiles of one operand and 4 of the other out of its L2.
+constexpr int kDown = 8;
+__device__ __forceinline__ bool place_tile(int id, int m_tiles, int n_tiles, int *m, int *n) {
+  const int tiles = m_tiles * n_tiles, per = (tiles + kXcds - 1) / kXcds;
+  const int t = (id % kXcds) * per + id / kXcds;
+  if (id / kXcds >= per || t >= tiles) return false;
+  const int group = t / (kDown * n_tiles), in = t - group * (kDown * n_tiles);
+  const int high = min(kDown, m_tiles - group * kDown);
+  *n = in / high;
+  *m = group * kDown + in - *n * high;
+  return true;
+}
+
+// How many m-tiles the experts have in all.
+__device__ __forceinline__ int count_tiles(const int32_t *offsets, int X, int64_t rows, int bm) {
+  int tiles = 0;
+  for (int e = lane_id(); e < X; e += kWave) {
+    const int64_t a = clamped(offsets, e, rows), b = clamped(offsets, e + 1, rows);
+    tiles += b > a ? (int)((b - a + bm - 1) / bm) : 0;
+  }
+#pragma unroll
+  for (int d = kWave / 2; d > 0; d >>= 1) tiles += __shfl_xor(tiles, d, kWave);
+  return __builtin_amdgcn_readfirstlane(tiles);
 }
 
 // The expert whose m-tile `tile` is, counted over all experts; its first row and the expert's last.  False: there is none.
@@ -173,14 +227,13 @@ __device__ __forceinline__ bool find_tile(const int32_t *offsets, int X, int64_t
     const uint64_t past = __ballot(before + s > tile);
     if (past) {
       const int w = __ffsll((unsigned long long)past) - 1;
-      const int first = before + __shfl(s - tiles, w, kWave);
-      *e = __builtin_amdgcn_readfirstlane(e0 + w);
-      const int64_t ea = clamped(offsets, *e, rows), eb = clamped(offsets, *e + 1, rows);
-      *r0 = ea + (int64_t)__builtin_amdgcn_readfirstlane(tile - first) * bm;
-      *r1 = eb;
+      const int first = before + __builtin_amdgcn_readlane(s - tiles, w);
+      *e = e0 + w;
+      *r0 = same(__shfl(a, w, kWave)) + (int64_t)(tile - first) * bm;
+      *r1 = same(__shfl(b, w, kWave));
       return true;
     }
-    before += __shfl(s, kWave - 1, kWave);
+    before += __builtin_amdgcn_readlane(s, kWave - 1);
   }
   return false;
 }
@@ -200,44 +253,37 @@ __device__ __forceinline__ void store_four(TO *p, const typename Mfma<T>::Acc &a
   }
 }
 
-// A wave computes BM/WM x BN/WN of the tile, B's fragment as the first operand: a lane then holds four neighbouring
-// columns of one row of the result.
-template <class T, class TO, int KIND, int BM, int BN, int WM, int WN, bool FAST, bool ADD>
-__global__ __launch_bounds__(WM *WN *kWave) void experts_kernel(TO *__restrict__ C, const T *__restrict__ A, const T *__restrict__ B,
-                                                                const int32_t *__restrict__ offsets, ProductShape g) {
-  constexpr int NT = WM * WN * kWave;
-  constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
-  using TA = Tile<T, BM, KIND == kGradW, NT, FAST>;
-  using TB = Tile<T, BN, KIND != kForward, NT, FAST>;
-  using Acc = typename Mfma<T>::Acc;
-  using Frag = typename Mfma<T>::Frag;
-  __shared__ __align__(128) T a0[BM * kDepth];
-  __shared__ __align__(128) T b0[BN * kDepth];
-  __shared__ __align__(128) T a1[BM * kDepth];
-  __shared__ __align__(128) T b1[BN * kDepth];
+// All but the last N loads of this wave have arrived and its LDS reads are done; then the workgroup's barrier.
+template <int N>
+__device__ __forceinline__ void arrived() {
+  static_assert(N < 64, "the counter has six bits");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 
+// Where a workgroup's tile is, and its operands.
+template <int KIND, int BM, int BN, class T, class TO, class TA, class TB>
+__device__ __forceinline__ bool place_product(TA &ta, TB &tb, TO *&out, int64_t &m0, int64_t &n0, int64_t &m_end, int64_t &summed,
+                                              TO *C, const T *A, const T *B, const int32_t *offsets, const ProductShape &g, bool skip_empty) {
   const int id = (int)blockIdx.x;
-  int e;
-  int64_t m0, n0, m_end, summed;
-  TA ta;
-  TB tb;
-  TO *out;
+  int e, m, n;
   if (KIND == kGradW) {
-    const int per = g.m_tiles * g.n_tiles;
+    // block after block of dW, each dealt to all dies: the blocks' costs differ with their experts' rows
+    const int per = (g.m_tiles * g.n_tiles + kXcds - 1) / kXcds * kXcds;
     e = id / per;
-    const int t = id - e * per;
-    m0 = (int64_t)(t / g.n_tiles) * BM;
-    n0 = (int64_t)(t % g.n_tiles) * BN;
+    if (!place_tile(id - e * per, g.m_tiles, g.n_tiles, &m, &n)) return false;
+    m0 = (int64_t)m * BM;
+    n0 = (int64_t)n * BN;
     m_end = g.M;
     const int64_t ra = clamped(offsets, e, g.rows), rb = clamped(offsets, e + 1, g.rows);
-    summed = rb > ra ? rb - ra : 0;
-    if (ADD && summed == 0) return;
+    summed = same(rb > ra ? rb - ra : 0);
+    if (skip_empty && summed == 0) return false;
     ta.init(A + ra * g.ldA + m0, g.ldA, summed ? (summed - 1) * g.ldA + g.M - m0 : 0, summed, g.M - m0);
     tb.init(B + ra * g.ldB + n0, g.ldB, summed ? (summed - 1) * g.ldB + g.N - n0 : 0, summed, g.N - n0);
     out = C + (int64_t)e * g.blockC;
   } else {
-    if (!find_tile(offsets, g.X, g.rows, BM, id / g.n_tiles, &e, &m0, &m_end)) return;
-    n0 = (int64_t)(id % g.n_tiles) * BN;
+    if (!place_tile(id, count_tiles(offsets, g.X, g.rows, BM), g.n_tiles, &m, &n)) return false;
+    if (!find_tile(offsets, g.X, g.rows, BM, m, &e, &m0, &m_end)) return false;
+    n0 = (int64_t)n * BN;
     summed = g.K;
     ta.init(A + m0 * g.ldA, g.ldA, (m_end - m0 - 1) * g.ldA + g.K, summed, m_end - m0);
     const T *w = B + (int64_t)e * g.blockB;
@@ -247,45 +293,12 @@ __global__ __launch_bounds__(WM *WN *kWave) void experts_kernel(TO *__restrict__
       tb.init(w + n0, g.ldB, (g.K - 1) * g.ldB + g.N - n0, summed, g.N - n0);
     out = C;
   }
+  return true;
+}
 
-  const int wm = wave_id() / WN, wn = wave_id() % WN;
-  Acc acc[NI][MI] = {};
-  const auto step = [&](const T *sa, const T *sb, T *na, T *nb, int64_t k0) {
-    __syncthreads();  // this step's slices have arrived, and nobody reads the other buffer any more
-    const bool more = k0 + kDepth < summed;
-    if (more) {
-      ta.bring(na, k0 + kDepth);
-      tb.bring(nb, k0 + kDepth);
-    }
-#pragma unroll
-    for (int kk = 0; kk < kDepth / 32; kk++) {
-      Frag fa[MI], fb[NI];
-#pragma unroll
-      for (int i = 0; i < MI; i++) fa[i] = TA::fragment(sa, wm * (BM / WM) + i * 16, kk);
-#pragma unroll
-      for (int j = 0; j < NI; j++) fb[j] = TB::fragment(sb, wn * (BN / WN) + j * 16, kk);
-#pragma unroll
-      for (int j = 0; j < NI; j++)
-#pragma unroll
-        for (int i = 0; i < MI; i++) acc[j][i] = Mfma<T>::go(fb[j], fa[i], acc[j][i]);
-    }
-    if (more) {
-      ta.put(na);
-      tb.put(nb);
-    }
-  };
-  if (summed > 0) {
-    ta.bring(a0, 0);
-    tb.bring(b0, 0);
-    ta.put(a0);
-    tb.put(b0);
-  }
-  for (int64_t k0 = 0; k0 < summed; k0 += 2 * kDepth) {
-    step(a0, b0, a1, b1, k0);
-    if (k0 + kDepth < summed) step(a1, b1, a0, b0, k0 + kDepth);
-  }
-
-  const int l = lane_id();
+template <class T, class TO, bool ADD, int BM, int BN, int WM, int WN, class Acc, int NI, int MI>
+__device__ __forceinline__ void store_product(TO *out, const Acc (&acc)[NI][MI], int64_t m0, int64_t n0, int64_t m_end, const ProductShape &g) {
+  const int l = lane_id(), wm = wave_id() / WN, wn = wave_id() % WN;
 #pragma unroll
   for (int i = 0; i < MI; i++) {
     const int64_t m = m0 + wm * (BM / WM) + i * 16 + (l & 15);
@@ -296,6 +309,146 @@ __global__ __launch_bounds__(WM *WN *kWave) void experts_kernel(TO *__restrict__
       if (n < g.N) store_four<T, TO, ADD>(out + m * g.ldC + n, acc[j][i], g.N - n);
     }
   }
+}
+
+// Any strides and alignment: the next step's chunks wait in registers while this one's products run.
+// A wave computes BM/WM x BN/WN of the tile, B's fragment as the first operand: a lane then holds four neighbouring
+// columns of one row of the result.
+template <class T, class TO, int KIND, int BM, int BN, int WM, int WN, bool ADD>
+__global__ __launch_bounds__(WM *WN *kWave) void experts_any_kernel(TO *__restrict__ C, const T *__restrict__ A, const T *__restrict__ B,
+                                                                    const int32_t *__restrict__ offsets, ProductShape g) {
+  constexpr int NT = WM * WN * kWave, DEPTH = 64;
+  constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
+  using TA = Tile<T, BM, DEPTH, KIND == kGradW, NT, false>;
+  using TB = Tile<T, BN, DEPTH, KIND != kForward, NT, false>;
+  using Acc = typename Mfma<T>::Acc;
+  using Frag = typename Mfma<T>::Frag;
+  __shared__ __align__(128) T sa[2][BM * DEPTH];
+  __shared__ __align__(128) T sb[2][BN * DEPTH];
+  TA ta;
+  TB tb;
+  TO *out;
+  int64_t m0, n0, m_end, summed;
+  if (!place_product<KIND, BM, BN>(ta, tb, out, m0, n0, m_end, summed, C, A, B, offsets, g, ADD)) return;
+  const int wm = wave_id() / WN, wn = wave_id() % WN;
+  Acc acc[NI][MI] = {};
+  if (summed > 0) {
+    ta.bring(0);
+    tb.bring(0);
+    ta.put(sa[0]);
+    tb.put(sb[0]);
+  }
+  int at = 0;
+  for (int64_t k0 = 0; k0 < summed; k0 += DEPTH, at ^= 1) {
+    __syncthreads();  // this step's slices are there, and nobody reads the other buffer any more
+    const bool more = k0 + DEPTH < summed;
+    if (more) {
+      ta.bring(k0 + DEPTH);
+      tb.bring(k0 + DEPTH);
+    }
+#pragma unroll
+    for (int kk = 0; kk < DEPTH / 32; kk++) {
+      Frag fa[MI], fb[NI];
+#pragma unroll
+      for (int i = 0; i < MI; i++) fa[i] = TA::fragment(sa[at], wm * (BM / WM) + i * 16, kk);
+#pragma unroll
+      for (int j = 0; j < NI; j++) fb[j] = TB::fragment(sb[at], wn * (BN / WN) + j * 16, kk);
+#pragma unroll
+      for (int j = 0; j < NI; j++)
+#pragma unroll
+        for (int i = 0; i < MI; i++) acc[j][i] = Mfma<T>::go(fb[j], fa[i], acc[j][i]);
+    }
+    if (more) {
+      ta.put(sa[at ^ 1]);
+      tb.put(sb[at ^ 1]);
+    }
+  }
+  store_product<T, TO, ADD, BM, BN, WM, WN>(out, acc, m0, n0, m_end, g);
+}
+
+// Rows that begin on 16 bytes.  Four stages of LDS, each DEPTH of the summed index: a stage's loads are started three steps
+// before its products.  A step of a wave: read this stage's fragments, start the loads of the stage three on, wait for
+// the fragments and for its own loads of the next stage (not for the later ones: vmcnt counts down in order), barrier, products.
+// Behind the barrier every wave's loads of the next stage are there, and the stage before this one may be overwritten.
+// Loads behind the end of the summed index are started like any others, read nothing and write zeros, so that the
+// number of loads in flight, which the wait counts, is always the same.
+//
+// With eight waves, two on each SIMD, waves 4 to 7 run one barrier behind waves 0 to 3 and every step has a second
+// barrier behind its products: while one wave of a SIMD feeds the matrix cores the other reads LDS, and they change places.
+// A stage is then read half a step later by the second four, still before the barrier behind which it is overwritten.
+template <class T, class TO, int KIND, int BM, int BN, int DEPTH, int WM, int WN, bool ADD>
+__global__ __launch_bounds__(WM *WN *kWave) void experts_kernel(TO *__restrict__ C, const T *__restrict__ A, const T *__restrict__ B,
+                                                                const int32_t *__restrict__ offsets, ProductShape g) {
+  constexpr int NT = WM * WN * kWave, S = 4, KK = DEPTH / 32;
+  constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
+  constexpr bool kPairs = WM * WN == 8;
+  using TA = Tile<T, BM, DEPTH, KIND == kGradW, NT, true>;
+  using TB = Tile<T, BN, DEPTH, KIND != kForward, NT, true>;
+  using Acc = typename Mfma<T>::Acc;
+  using Frag = typename Mfma<T>::Frag;
+  constexpr int L = TA::kLoads + TB::kLoads;
+  // an array for each stage: what is read from one does not wait for loads into another
+  __shared__ __align__(128) T a0[BM * DEPTH], a1[BM * DEPTH], a2[BM * DEPTH], a3[BM * DEPTH];
+  __shared__ __align__(128) T b0[BN * DEPTH], b1[BN * DEPTH], b2[BN * DEPTH], b3[BN * DEPTH];
+  TA ta;
+  TB tb;
+  TO *out;
+  int64_t m0, n0, m_end, summed;
+  if (!place_product<KIND, BM, BN>(ta, tb, out, m0, n0, m_end, summed, C, A, B, offsets, g, ADD)) return;
+  const int wm = wave_id() / WN, wn = wave_id() % WN;
+  Acc acc[NI][MI] = {};
+  // the products of stage t, which is in sa, sb; na, nb take the stage three on
+  const auto step = [&](const T *sa, const T *sb, T *na, T *nb, int t) {
+    Frag fa[KK][MI], fb[KK][NI];
+#pragma unroll
+    for (int kk = 0; kk < KK; kk++) {
+#pragma unroll
+      for (int j = 0; j < NI; j++) fb[kk][j] = TB::fragment(sb, wn * (BN / WN) + j * 16, kk);
+#pragma unroll
+      for (int i = 0; i < MI; i++) fa[kk][i] = TA::fragment(sa, wm * (BM / WM) + i * 16, kk);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    ta.start(na, t + S - 1);
+    tb.start(nb, t + S - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    arrived<(S - 2) * L>();
+    __builtin_amdgcn_sched_barrier(0);
+    if (kPairs) __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+      for (int j = 0; j < NI; j++)
+#pragma unroll
+        for (int i = 0; i < MI; i++) acc[j][i] = Mfma<T>::go(fb[kk][j], fa[kk][i], acc[j][i]);
+    if (kPairs) {
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  if (summed > 0) {
+    ta.start(a0, 0);
+    tb.start(b0, 0);
+    ta.start(a1, 1);
+    tb.start(b1, 1);
+    ta.start(a2, 2);
+    tb.start(b2, 2);
+    arrived<(S - 2) * L>();
+    const bool second = kPairs && wave_id() >= 4;
+    if (second) __builtin_amdgcn_s_barrier();
+    for (int64_t k0 = 0; k0 < summed; k0 += S * DEPTH) {  // steps behind the last multiply zeros
+      step(a0, b0, a3, b3, 0);
+      step(a1, b1, a0, b0, 1);
+      step(a2, b2, a1, b1, 2);
+      step(a3, b3, a2, b2, 3);
+      ta.move(S);
+      tb.move(S);
+    }
+    if (kPairs && !second) __builtin_amdgcn_s_barrier();  // as many barriers as the others
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // no load may still write to LDS when the workgroup has ended
+  }
+  store_product<T, TO, ADD, BM, BN, WM, WN>(out, acc, m0, n0, m_end, g);
 }
 
 }  // namespace tok
