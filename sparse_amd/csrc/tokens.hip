@@ -148,21 +148,22 @@ struct GradPlan {
   bool small;
   int passes, bits;
   Split split;
-  uint32_t *keys, *keys2, *clear, *marks;
+  uint32_t *keys, *keys2;
   int32_t *items, *items2;
-  int *hist, *next_hist;
+  int *hist;
   float *part;
-  int64_t clear_words, mark_words, bytes;
+  uint8_t *named;
+  int64_t bytes;
 
   GradPlan(void *work, int type, int64_t n, int64_t V, int64_t D) : split(n > 0 ? n : 1) {
     const int64_t per = 16 / type_size(type);
+    g = {};
     g.n = n; g.V = V; g.D = D;
     g.segs = cdiv(cdiv(D, per), kWave);
     // chunks of 32 read a key, an item and two chunk ends for 32 rows; where that leaves the card empty, chunks of 8
     g.chunk = cdiv(n, 32) * g.segs >= kFullCard ? 32 : 8;
     g.chunks = cdiv(n, g.chunk);
-    mark_words = cdiv(V, 32);
-    small = n <= kOneGroup && mark_words <= ((int64_t)1 << 17);
+    small = n <= kOneGroupIds && V <= ((int64_t)1 << 22);  // one workgroup clears the rows' bytes too
     const int key_bits = bits_for(V + 1) > 0 ? bits_for(V + 1) : 1;
     const int most = small ? kSmallBits : 10;
     passes = (key_bits + most - 1) / most;
@@ -170,19 +171,10 @@ struct GradPlan {
     Carve c(work);
     keys = c.take<uint32_t>(n);
     items = c.take<int32_t>(n);
-    keys2 = nullptr; items2 = nullptr; hist = nullptr; next_hist = nullptr; clear = nullptr; clear_words = 0;
-    if (small) {
-      marks = c.take<uint32_t>(mark_words);
-    } else {
-      keys2 = c.take<uint32_t>(n);
-      items2 = c.take<int32_t>(n);
-      const int64_t counts = (int64_t)split.groups << bits;
-      hist = c.take<int>(counts);
-      clear_words = counts * (passes - 1) + mark_words;  // later passes' counts, then the marks
-      clear = c.take<uint32_t>(clear_words);
-      next_hist = (int *)clear;
-      marks = clear ? clear + counts * (passes - 1) : nullptr;
-    }
+    keys2 = small ? nullptr : c.take<uint32_t>(n);
+    items2 = small ? nullptr : c.take<int32_t>(n);
+    hist = small ? nullptr : c.take<int>((int64_t)split.groups << bits);
+    named = c.take<uint8_t>(cdiv(V, 4) * 4);
     part = c.take<float>(g.chunks > 1 ? g.chunks * 2 * g.segs * kWave * per : 0);
     bytes = c.used;
   }
@@ -196,58 +188,79 @@ int check_work(futhark_context *ctx, const char *who, const void *work, int64_t 
 }
 
 template <class I>
-int order_ids(futhark_context *ctx, hipStream_t stream, const I *ids, const GradPlan &p, bool marked) {
-  uint32_t *marks = marked ? p.marks : nullptr;
+int order_ids(futhark_context *ctx, hipStream_t stream, const I *ids, const GradPlan &p, bool mark) {
+  uint8_t *named = mark ? p.named : nullptr;
   const int n = (int)p.g.n;
   if (p.small) {
     if (n <= 1024)
-      TOK_LAUNCH(ctx, (id_sort_small_kernel<I, 1>), 1, 1024, stream, ids, n, p.g.V, p.passes, p.bits, p.keys, p.items, marks, p.mark_words);
-    else if (n <= 4096)
-      TOK_LAUNCH(ctx, (id_sort_small_kernel<I, 4>), 1, 1024, stream, ids, n, p.g.V, p.passes, p.bits, p.keys, p.items, marks, p.mark_words);
+      TOK_LAUNCH(ctx, (id_sort_small_kernel<I, 1>), 1, 1024, stream, ids, n, p.g.V, p.passes, p.bits, p.keys, p.items, named);
     else
-      TOK_LAUNCH(ctx, (id_sort_small_kernel<I, 8>), 1, 1024, stream, ids, n, p.g.V, p.passes, p.bits, p.keys, p.items, marks, p.mark_words);
+      TOK_LAUNCH(ctx, (id_sort_small_kernel<I, 2>), 1, 1024, stream, ids, n, p.g.V, p.passes, p.bits, p.keys, p.items, named);
     return 0;
   }
   const int bins = 1 << p.bits, mask = bins - 1;
-  const int64_t counts = (int64_t)p.split.groups << p.bits;
-  const Digits<1, I> d0 = {ids, nullptr, p.g.n, p.g.V, 0, mask};
-  TOK_LAUNCH(ctx, (digit_count_kernel<1, I>), p.split.groups, kThreads, stream, d0, p.split.per_group, bins, p.hist, p.clear, p.clear_words);
   for (int k = 0; k < p.passes; k++) {
-    const bool last = k == p.passes - 1, to_first = (p.passes - 1 - k) % 2 == 0;
+    const bool to_first = (p.passes - 1 - k) % 2 == 0;
     PassOut o = {};
     o.keys = to_first ? p.keys : p.keys2;
     o.items = to_first ? p.items : p.items2;
-    if (!last) {
-      o.next_hist = p.next_hist + counts * k;
-      o.next_shift = (k + 1) * p.bits;
-      o.next_mask = mask;
-      o.next_bins = bins;
-    }
     if (k == 0) {
-      o.marks = marks;
-      TOK_LAUNCH(ctx, (digit_place_kernel<1, I>), p.split.groups, kThreads, stream, d0, p.split.per_group, bins, p.bits, (const int *)p.hist, o);
+      const Digits<1, I> d = {ids, nullptr, p.g.n, p.g.V, 0, mask};
+      o.named = named;
+      TOK_LAUNCH(ctx, (digit_count_kernel<1, I>), p.split.groups, kSplitThreads, stream, d, p.split.per_group, bins, p.hist,
+                 (uint32_t *)named, named ? cdiv(p.g.V, 4) : 0);
+      TOK_LAUNCH(ctx, (digit_place_kernel<1, I>), p.split.groups, kSplitThreads, stream, d, p.split.per_group, bins, p.bits, (const int *)p.hist, o);
     } else {
       o.items_in = to_first ? p.items2 : p.items;
       const Digits<2, I> d = {nullptr, to_first ? p.keys2 : p.keys, p.g.n, p.g.V, k * p.bits, mask};
-      TOK_LAUNCH(ctx, (digit_place_kernel<2, I>), p.split.groups, kThreads, stream, d, p.split.per_group, bins, p.bits,
-                 (const int *)(p.next_hist + counts * (k - 1)), o);
+      TOK_LAUNCH(ctx, (digit_count_kernel<2, I>), p.split.groups, kSplitThreads, stream, d, p.split.per_group, bins, p.hist,
+                 (uint32_t *)nullptr, (int64_t)0);
+      TOK_LAUNCH(ctx, (digit_place_kernel<2, I>), p.split.groups, kSplitThreads, stream, d, p.split.per_group, bins, p.bits, (const int *)p.hist, o);
     }
   }
   return 0;
 }
 
-template <class T, class TO, bool ADD>
+template <class T, class TO, bool ADD, bool STREAM>
 int sum_ids(futhark_context *ctx, hipStream_t stream, TO *dE, const T *dy, const float *vals, float scale, GradPlan &p) {
-  const int64_t fill_units = cdiv(p.g.D, kPer<TO>);
-  p.g.fill_segs = ADD ? 0 : cdiv(fill_units, kWave * kFillPieces);
-  const int64_t blocks = cdiv(p.g.chunks * p.g.segs + p.g.V * p.g.fill_segs, kWaves);
+  if (!ADD) p.g.fill = deal_rows(p.g.V, cdiv(p.g.D, kPer<TO>), kFillPieces);
+  const int64_t blocks = cdiv(p.g.chunks * p.g.segs + p.g.fill.waves, kWaves);
   SAMD_TRY(check_blocks(ctx, "lookup_grad", blocks));
   SAMD_TRY(check_blocks(ctx, "lookup_grad", p.g.chunks * p.g.segs));
-  TOK_LAUNCH(ctx, (lookup_grad_kernel<T, TO, ADD>), blocks, kThreads, stream, dE, dy, vals, scale, (const uint32_t *)p.keys,
-             (const int32_t *)p.items, (const uint32_t *)p.marks, p.part, p.g);
+  TOK_LAUNCH(ctx, (lookup_grad_kernel<T, TO, ADD, STREAM>), blocks, kThreads, stream, dE, dy, vals, scale, (const uint32_t *)p.keys,
+             (const int32_t *)p.items, (const uint8_t *)p.named, p.part, p.g);
   if (p.g.chunks > 1)
-    TOK_LAUNCH(ctx, (lookup_grad_join_kernel<T, TO, ADD>), p.g.chunks * p.g.segs, kThreads, stream, dE, (const uint32_t *)p.keys, p.part, p.g);
+    TOK_LAUNCH(ctx, (lookup_grad_join_kernel<T, TO, ADD, STREAM>), p.g.chunks * p.g.segs, kThreads, stream, dE, (const uint32_t *)p.keys, p.part, p.g);
   return 0;
+}
+
+template <class T, class TO, class I, bool ADD, bool STREAM>
+int sum_few(futhark_context *ctx, hipStream_t stream, TO *dE, const T *dy, const I *ids, const float *vals, float scale, GradShape g) {
+  const int64_t units = cdiv(g.D, kPer<TO>);
+  g.fill = deal_rows(1, units, 1);
+  // 16 to 128 KiB of zeros for a workgroup: two of them on every CU if there is that much
+  const int64_t share = g.V * units * 16 / 512;
+  const int64_t rows = (share < 16 * 1024 ? 16 * 1024 : share > 128 * 1024 ? 128 * 1024 : share) / (units * 16);
+  const int fill_rows = (int)(rows < 1 ? 1 : rows > kFewFillRows ? kFewFillRows : rows);
+  const int64_t blocks = g.segs + (ADD ? 0 : cdiv(g.V, fill_rows));
+  SAMD_TRY(check_blocks(ctx, "lookup_grad", blocks));
+  TOK_LAUNCH(ctx, (lookup_grad_few_kernel<T, TO, I, ADD, STREAM>), blocks, kFewWaves * kWave, stream, dE, dy, ids, vals, scale, g, fill_rows);
+  return 0;
+}
+
+template <class T, class TO, class I>
+int sum_few_as(futhark_context *ctx, hipStream_t stream, bool add, TO *dE, const T *dy, const I *ids, const float *vals, float scale, const GradShape &g) {
+  if (add) return sum_few<T, TO, I, true, false>(ctx, stream, dE, dy, ids, vals, scale, g);
+  if (g.V * g.D * (int64_t)sizeof(TO) > kStreamBytes) return sum_few<T, TO, I, false, true>(ctx, stream, dE, dy, ids, vals, scale, g);
+  return sum_few<T, TO, I, false, false>(ctx, stream, dE, dy, ids, vals, scale, g);
+}
+
+// The gradient's table: written past the caches when all of it is written and it is large.
+template <class T, class TO>
+int sum_ids_as(futhark_context *ctx, hipStream_t stream, bool add, TO *dE, const T *dy, const float *vals, float scale, GradPlan &p) {
+  if (add) return sum_ids<T, TO, true, false>(ctx, stream, dE, dy, vals, scale, p);
+  if (p.g.V * p.g.D * (int64_t)sizeof(TO) > kStreamBytes) return sum_ids<T, TO, false, true>(ctx, stream, dE, dy, vals, scale, p);
+  return sum_ids<T, TO, false, false>(ctx, stream, dE, dy, vals, scale, p);
 }
 
 // ---------------------------------------------------------------- experts
@@ -329,11 +342,12 @@ int sparse_amd_tokens_lookup(struct futhark_context *ctx, void *stream, int type
         const int u = d.lg == 6 && d.waves >= kFullCard ? 4 : 1;
         if (u == 1) d = deal_rows(n, units, 1);
         SAMD_TRY(check_blocks(ctx, who, cdiv(d.waves, kWaves)));
-        if (u == 4)
-          TOK_LAUNCH(ctx, (lookup_kernel<T, I, 4>), cdiv(d.waves, kWaves), kThreads, s, (T *)y, ldy, (const T *)table, ldt, V, D, (const I *)ids, n, vals, scale, d.lg, d.segs);
-        else
-          TOK_LAUNCH(ctx, (lookup_kernel<T, I, 1>), cdiv(d.waves, kWaves), kThreads, s, (T *)y, ldy, (const T *)table, ldt, V, D, (const I *)ids, n, vals, scale, d.lg, d.segs);
-        return 0;
+        const auto go = [&](auto kernel) -> int {
+          TOK_LAUNCH(ctx, kernel, cdiv(d.waves, kWaves), kThreads, s, (T *)y, ldy, (const T *)table, ldt, V, D, (const I *)ids, n, vals, scale, d.lg, d.segs);
+          return 0;
+        };
+        if (n * D * (int64_t)sizeof(T) > kStreamBytes) return u == 4 ? go(lookup_kernel<T, I, 4, true>) : go(lookup_kernel<T, I, 1, true>);
+        return u == 4 ? go(lookup_kernel<T, I, 4, false>) : go(lookup_kernel<T, I, 1, false>);
       });
     });
   });
@@ -360,7 +374,7 @@ int sparse_amd_tokens_lookup_dots(struct futhark_context *ctx, void *stream, int
 }
 
 int64_t sparse_amd_tokens_lookup_grad_workspace(int type, int64_t n, int64_t V, int64_t D) {
-  if (n <= 0 || V < 0 || D <= 0) return 0;
+  if (n <= 0 || (n <= kFewIds && V <= kFewTable) || V < 0 || D <= 0) return 0;
   return GradPlan(nullptr, type, n, V, D).bytes;
 }
 
@@ -381,23 +395,24 @@ int sparse_amd_tokens_lookup_grad(struct futhark_context *ctx, void *stream, int
                                             {"the workspace", work, 1, work ? work_bytes : 0, work_bytes, 1}}));
         if (V == 0 || D == 0 || (n == 0 && accumulate)) return 0;
         const hipStream_t s = (hipStream_t)stream;
-        GradPlan p(n > 0 ? work : nullptr, type, n, V, D);
-        if (n > 0) SAMD_TRY(check_work(ctx, who, work, work_bytes, p.bytes));
+        GradPlan p(work, type, n, V, D);
         p.g.ldy = ldy;
         p.g.ldE = ldt;
-        if (n > 0) SAMD_TRY(order_ids<I>(ctx, s, (const I *)ids, p, !accumulate));  // without ids there are no marks: all rows are zeroed
-        if (out_type == type)
-          return accumulate ? sum_ids<T, T, true>(ctx, s, (T *)dtable, (const T *)dy, vals, scale, p)
-                            : sum_ids<T, T, false>(ctx, s, (T *)dtable, (const T *)dy, vals, scale, p);
-        return accumulate ? sum_ids<T, float, true>(ctx, s, (float *)dtable, (const T *)dy, vals, scale, p)
-                          : sum_ids<T, float, false>(ctx, s, (float *)dtable, (const T *)dy, vals, scale, p);
+        if (n == 0 || (n <= kFewIds && V <= kFewTable)) {
+          if (out_type == type) return sum_few_as<T, T, I>(ctx, s, accumulate != 0, (T *)dtable, (const T *)dy, (const I *)ids, vals, scale, p.g);
+          return sum_few_as<T, float, I>(ctx, s, accumulate != 0, (float *)dtable, (const T *)dy, (const I *)ids, vals, scale, p.g);
+        }
+        SAMD_TRY(check_work(ctx, who, work, work_bytes, p.bytes));
+        SAMD_TRY(order_ids<I>(ctx, s, (const I *)ids, p, !accumulate));
+        if (out_type == type) return sum_ids_as<T, T>(ctx, s, accumulate != 0, (T *)dtable, (const T *)dy, vals, scale, p);
+        return sum_ids_as<T, float>(ctx, s, accumulate != 0, (float *)dtable, (const T *)dy, vals, scale, p);
       });
     });
   });
 }
 
 int64_t sparse_amd_tokens_route_workspace(int64_t n, int64_t X) {
-  if (n <= kOneGroup || X < 1) return 0;
+  if (n <= kOneGroupChoices || X < 1) return 0;
   return (Split(n).groups * (X + 1) * (int64_t)sizeof(int) + 255) & ~(int64_t)255;
 }
 
@@ -417,16 +432,16 @@ int sparse_amd_tokens_route(struct futhark_context *ctx, void *stream, const voi
         TOK_LAUNCH(ctx, (route_small_kernel<I, 4, 1>), 1, 256, s, (const I *)chosen, (int)n, (int)X, bits, pos, src, offsets);
       else if (n <= 1024)
         TOK_LAUNCH(ctx, (route_small_kernel<I, 16, 1>), 1, 1024, s, (const I *)chosen, (int)n, (int)X, bits, pos, src, offsets);
-      else if (n <= kOneGroup)
-        TOK_LAUNCH(ctx, (route_small_kernel<I, 16, 8>), 1, 1024, s, (const I *)chosen, (int)n, (int)X, bits, pos, src, offsets);
+      else if (n <= kOneGroupChoices)
+        TOK_LAUNCH(ctx, (route_small_kernel<I, 16, 4>), 1, 1024, s, (const I *)chosen, (int)n, (int)X, bits, pos, src, offsets);
       else {
         SAMD_TRY(check_work(ctx, who, work, work_bytes, sparse_amd_tokens_route_workspace(n, X)));
         const Split sp(n);
         const Digits<0, I> d = {(const I *)chosen, nullptr, n, X, 0, 0};
-        TOK_LAUNCH(ctx, (digit_count_kernel<0, I>), sp.groups, kThreads, s, d, sp.per_group, (int)X + 1, (int *)work, (uint32_t *)nullptr, (int64_t)0);
+        TOK_LAUNCH(ctx, (digit_count_kernel<0, I>), sp.groups, kSplitThreads, s, d, sp.per_group, (int)X + 1, (int *)work, (uint32_t *)nullptr, (int64_t)0);
         PassOut o = {};
         o.pos = pos; o.src = src; o.offsets = offsets;
-        TOK_LAUNCH(ctx, (digit_place_kernel<0, I>), sp.groups, kThreads, s, d, sp.per_group, (int)X + 1, bits, (const int *)work, o);
+        TOK_LAUNCH(ctx, (digit_place_kernel<0, I>), sp.groups, kSplitThreads, s, d, sp.per_group, (int)X + 1, bits, (const int *)work, o);
       }
       return 0;
     });
@@ -449,11 +464,12 @@ int sparse_amd_tokens_dispatch(struct futhark_context *ctx, void *stream, int ty
       const int u = d.lg == 6 && d.waves >= kFullCard ? 4 : 1;
       if (u == 1) d = deal_rows(n, units, 1);
       SAMD_TRY(check_blocks(ctx, who, cdiv(d.waves, kWaves)));
-      if (u == 4)
-        TOK_LAUNCH(ctx, (dispatch_kernel<T, 4>), cdiv(d.waves, kWaves), kThreads, s, (T *)xs, ldxs, (const T *)x, ldx, n, D, (int)K, pos, slots, weights, d.lg, d.segs);
-      else
-        TOK_LAUNCH(ctx, (dispatch_kernel<T, 1>), cdiv(d.waves, kWaves), kThreads, s, (T *)xs, ldxs, (const T *)x, ldx, n, D, (int)K, pos, slots, weights, d.lg, d.segs);
-      return 0;
+      const auto go = [&](auto kernel) -> int {
+        TOK_LAUNCH(ctx, kernel, cdiv(d.waves, kWaves), kThreads, s, (T *)xs, ldxs, (const T *)x, ldx, n, D, (int)K, pos, slots, weights, d.lg, d.segs);
+        return 0;
+      };
+      if (n * K * D * (int64_t)sizeof(T) > kStreamBytes) return u == 4 ? go(dispatch_kernel<T, 4, true>) : go(dispatch_kernel<T, 1, true>);
+      return u == 4 ? go(dispatch_kernel<T, 4, false>) : go(dispatch_kernel<T, 1, false>);
     });
   });
 }
@@ -471,8 +487,11 @@ int sparse_amd_tokens_combine(struct futhark_context *ctx, void *stream, int typ
       const hipStream_t s = (hipStream_t)stream;
       const RowDeal d = deal_rows(n, cdiv(D, kPer<T>), 1);
       SAMD_TRY(check_blocks(ctx, who, cdiv(d.waves, kWaves)));
-      TOK_LAUNCH(ctx, (combine_kernel<T, 1>), cdiv(d.waves, kWaves), kThreads, s, (T *)y, ldy, (const T *)ys, ldys, n, D, (int)K, pos, slots, weights, d.lg, d.segs);
-      return 0;
+      const auto go = [&](auto kernel) -> int {
+        TOK_LAUNCH(ctx, kernel, cdiv(d.waves, kWaves), kThreads, s, (T *)y, ldy, (const T *)ys, ldys, n, D, (int)K, pos, slots, weights, d.lg, d.segs);
+        return 0;
+      };
+      return n * D * (int64_t)sizeof(T) > kStreamBytes ? go(combine_kernel<T, 1, true>) : go(combine_kernel<T, 1, false>);
     });
   });
 }
@@ -490,8 +509,11 @@ int sparse_amd_tokens_combine_grad(struct futhark_context *ctx, void *stream, in
                                           {"pos", pos, n, K, K, 4}, {"weights", weights, n, K, K, 4}}));
       if (n == 0 || K == 0) return 0;
       SAMD_TRY(check_blocks(ctx, who, n));
-      TOK_LAUNCH(ctx, (combine_grad_kernel<T>), n, kThreads, (hipStream_t)stream, (T *)dys, lddys, dweights, (const T *)dy, lddy, (const T *)ys, ldys, D, (int)K, pos, slots, weights);
-      return 0;
+      const auto go = [&](auto kernel) -> int {
+        TOK_LAUNCH(ctx, kernel, n, kThreads, (hipStream_t)stream, (T *)dys, lddys, dweights, (const T *)dy, lddy, (const T *)ys, ldys, D, (int)K, pos, slots, weights);
+        return 0;
+      };
+      return n * K * D * (int64_t)sizeof(T) > kStreamBytes ? go(combine_grad_kernel<T, true>) : go(combine_grad_kernel<T, false>);
     });
   });
 }

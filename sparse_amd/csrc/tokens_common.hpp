@@ -25,42 +25,67 @@ struct Piece {
   T v[kPer<T>];
 };
 
-// The `left` elements (kPer or fewer) of a piece at p; what is not there reads as zero.
-template <class T>
+typedef uint32_t __attribute__((ext_vector_type(4), aligned(2))) Quad;  // 16 bytes at any element's address
+
+// The `left` elements (kPer or fewer) of a piece at p; what is not there reads as zero.  ONCE: nobody will read them again
+// soon, so they are not kept in the caches in the place of what will be (a non-temporal load).
+template <bool ONCE = false, class T>
 __device__ __forceinline__ Piece<T> load_piece(const T *p, int64_t left) {
-  Piece<T> r;
+  Piece<T> r = {};
   if (left >= kPer<T>) {
-    __builtin_memcpy(&r, p, 16);
-  } else {
+    if (ONCE) {
+      const Quad q = __builtin_nontemporal_load((const Quad *)p);
+      __builtin_memcpy(&r, &q, 16);
+    } else {
+      __builtin_memcpy(&r, p, 16);
+    }
+  } else if (left > 0) {
 #pragma unroll
-    for (int i = 0; i < kPer<T>; i++) r.v[i] = i < left ? p[i] : (T)0.0f;
+    for (int i = 0; i < kPer<T> - 1; i++)
+      if (i < left) r.v[i] = p[i];
   }
   return r;
 }
 
-template <class T>
+template <bool STREAM = false, class T>
 __device__ __forceinline__ void store_piece(T *p, const Piece<T> &r, int64_t left) {
   if (left >= kPer<T>) {
-    __builtin_memcpy(p, &r, 16);
-  } else {
+    if (STREAM) {
+      Quad q;
+      __builtin_memcpy(&q, &r, 16);
+      __builtin_nontemporal_store(q, (Quad *)p);
+    } else {
+      __builtin_memcpy(p, &r, 16);
+    }
+  } else if (left > 0) {
 #pragma unroll
-    for (int i = 0; i < kPer<T>; i++)
+    for (int i = 0; i < kPer<T> - 1; i++)
       if (i < left) p[i] = r.v[i];
   }
 }
 
+// A result larger than the L2s of the card (8 x 4 MiB) is written past them: its lines would push out each other and what
+// is being read (non-temporal stores; 16384 rows of 8 KiB looked up: 45 -> 32 us, a gradient of 512 MiB: 157 -> 88 us).
+// A smaller one is left to the caches, where the next kernel finds it.
+constexpr int64_t kStreamBytes = (int64_t)32 << 20;
+
 // kPer<T> sums held in 32 bits, rounded once to TO (16 or 32 bits) and stored; ADD: added to what is there first.
-template <class T, class TO, bool ADD>
+template <class T, class TO, bool ADD, bool STREAM>
 __device__ __forceinline__ void store_sums(TO *p, const float (&s)[kPer<T>], int64_t left) {
   if (left >= kPer<T>) {
-    TO o[kPer<T>];
+    constexpr int n = kPer<T> / kPer<TO>;  // pieces of the result: one, or two of 32 bits from 16
+    Piece<TO> o[n];
     if (ADD) __builtin_memcpy(o, p, sizeof o);
 #pragma unroll
-    for (int i = 0; i < kPer<T>; i++) o[i] = (TO)(ADD ? (float)o[i] + s[i] : s[i]);
-    __builtin_memcpy(p, o, sizeof o);
-  } else {
+    for (int i = 0; i < kPer<T>; i++) {
+      TO &x = o[i / kPer<TO>].v[i % kPer<TO>];
+      x = (TO)(ADD ? (float)x + s[i] : s[i]);
+    }
 #pragma unroll
-    for (int i = 0; i < kPer<T>; i++)
+    for (int i = 0; i < n; i++) store_piece<STREAM>(p + i * kPer<TO>, o[i], kPer<TO>);
+  } else if (left > 0) {
+#pragma unroll
+    for (int i = 0; i < kPer<T> - 1; i++)
       if (i < left) p[i] = (TO)(ADD ? (float)p[i] + s[i] : s[i]);
   }
 }
@@ -74,6 +99,9 @@ __device__ __forceinline__ float wave_sum(float v) {
 __device__ __forceinline__ int lane_id() { return (int)(threadIdx.x & (kWave - 1)); }
 // The same in every lane of a wave, and known to be: what is indexed by it is loaded once per wave.
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave)); }
+
+// Among the waves of a launch of kThreads threads a workgroup.
+__device__ __forceinline__ int64_t wave_number() { return (int64_t)blockIdx.x * kWaves + wave_id(); }
 
 // How a launch deals rows to waves.  Rows of 64 pieces or more: a wave takes `u` x 64 pieces of one row, `segs` waves a
 // row.  Shorter rows: a power of two of lanes each (1 << lg), so that a wave takes several.
@@ -96,8 +124,8 @@ struct RowPlace {
   int64_t row, unit;  // this lane's row, and its first piece in it
 };
 
-__device__ __forceinline__ RowPlace my_row(int lg, int64_t segs, int u) {
-  const int64_t w = (int64_t)blockIdx.x * kWaves + wave_id();
+// of the w-th wave of such a launch
+__device__ __forceinline__ RowPlace my_row(int64_t w, int lg, int64_t segs, int u) {
   const int lane = lane_id();
   RowPlace r;
   if (lg == 6) {

@@ -17,10 +17,10 @@ namespace tok {
 struct GradShape {
   int64_t n, V, D;
   int64_t ldy, ldE;
-  int64_t segs;       // waves along a row of dy, 64 pieces each
+  int64_t segs;      // waves along a row of dy, 64 pieces each
   int64_t chunks;
-  int64_t fill_segs;  // waves along a row of dE that is zeroed; 0: none are
-  int chunk;          // positions in a chunk: a multiple of 8
+  RowDeal fill;      // of the rows that are zeroed; no waves when sums are added to what is there
+  int chunk;         // positions in a chunk: a multiple of 8
 };
 
 constexpr int kFillPieces = 4;
@@ -31,25 +31,25 @@ __device__ __forceinline__ float *chunk_sum(float *part, const GradShape &g, int
   return part + ((chunk * 2 + tail) * g.segs * kWave + unit) * kPer<T>;
 }
 
-template <class T, class TO, bool ADD>
+template <class T, class TO, bool ADD, bool STREAM>
 __global__ __launch_bounds__(kThreads) void lookup_grad_kernel(TO *__restrict__ dE, const T *__restrict__ dy,
                                                                const float *__restrict__ vals, float scale,
                                                                const uint32_t *__restrict__ keys, const int32_t *__restrict__ items,
-                                                               const uint32_t *__restrict__ marks, float *__restrict__ part,
+                                                               const uint8_t *__restrict__ named, float *__restrict__ part,
                                                                GradShape g) {
   constexpr int R = 8;
   const int64_t w = (int64_t)blockIdx.x * kWaves + wave_id();
   const int lane = lane_id();
   const int64_t chunk = w / g.segs;
-  if (chunk >= g.chunks) {  // zero the rows no id names
-    if (ADD || g.fill_segs == 0) return;
-    const int64_t f = w - g.chunks * g.segs, row = f / g.fill_segs;
-    if (row >= g.V || (marks && ((marks[row >> 5] >> (row & 31)) & 1))) return;
-    Piece<TO> z = {};
+  if (chunk >= g.chunks) {  // zero the rows no id names (named: a byte for each row)
+    if (ADD) return;
+    const RowPlace at = my_row(w - g.chunks * g.segs, g.fill.lg, g.fill.segs, kFillPieces);
+    if (at.row >= g.V || named[at.row]) return;
+    const Piece<TO> z = {};
 #pragma unroll
     for (int u = 0; u < kFillPieces; u++) {
-      const int64_t c = (((f - row * g.fill_segs) * kFillPieces + u) * kWave + lane) * kPer<TO>;
-      if (c < g.D) store_piece(dE + row * g.ldE + c, z, g.D - c);
+      const int64_t c = (at.unit + u * kWave) * kPer<TO>;
+      if (c < g.D) store_piece<STREAM>(dE + at.row * g.ldE + c, z, g.D - c);
     }
     return;
   }
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_kernel(TO *__restrict__ 
       k[r] = p + r < p1 ? keys[p + r] : none;
       const int64_t i = k[r] != none ? items[p + r] : 0;
       f[r] = vals ? scale * vals[i] : scale;
-      x[r] = load_piece(dy + i * g.ldy + c, k[r] != none ? g.D - c : 0);
+      x[r] = load_piece<!STREAM>(dy + i * g.ldy + c, k[r] != none ? g.D - c : 0);
     }
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_kernel(TO *__restrict__ 
 #pragma unroll
             for (int i = 0; i < kPer<T>; i++) to[i] = s[i];
           } else {
-            store_sums<T, TO, ADD>(dE + (int64_t)run * g.ldE + c, s, g.D - c);
+            store_sums<T, TO, ADD, STREAM>(dE + (int64_t)run * g.ldE + c, s, g.D - c);
           }
         }
         run = k[r];
@@ -101,13 +101,13 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_kernel(TO *__restrict__ 
 #pragma unroll
     for (int i = 0; i < kPer<T>; i++) to[i] = s[i];
   } else {
-    store_sums<T, TO, ADD>(dE + (int64_t)run * g.ldE + c, s, g.D - c);
+    store_sums<T, TO, ADD, STREAM>(dE + (int64_t)run * g.ldE + c, s, g.D - c);
   }
 }
 
 // One workgroup for each chunk and 64 pieces: returns at once unless a run begins in the chunk and goes on behind it.
 // Its waves add a part of the run's chunk sums each, and the parts are added in order.
-template <class T, class TO, bool ADD>
+template <class T, class TO, bool ADD, bool STREAM>
 __global__ __launch_bounds__(kThreads) void lookup_grad_join_kernel(TO *__restrict__ dE, const uint32_t *__restrict__ keys,
                                                                     float *__restrict__ part, GradShape g) {
   __shared__ float sums[kWaves][kWave][kPer<T>];
@@ -116,19 +116,24 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_join_kernel(TO *__restri
   if (p1 >= g.n) return;
   const uint32_t run = keys[p1 - 1];
   if (run == (uint32_t)g.V || keys[p1] != run || (p0 > 0 && keys[p0 - 1] == run)) return;
-  int64_t lo = p1, hi = g.n;  // the end of the run: first position behind p1 with a larger key
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (keys[mid] <= run) lo = mid + 1; else hi = mid;
+  // chunk sums of the run: this chunk's tail, then the heads of the chunks that begin with it (64 chunks looked at at once)
+  int64_t count = 1;
+  for (;;) {
+    const int64_t q = (chunk + count + lane_id()) * g.chunk;
+    const uint64_t other = ~__ballot(q < g.n && keys[q] == run);
+    if (other) {
+      count += __builtin_ctzll(other);
+      break;
+    }
+    count += kWave;
   }
-  const int64_t count = (lo - 1) / g.chunk - chunk + 1;  // chunk sums of the run: this chunk's tail, then heads
   const int64_t each = (count + kWaves - 1) / kWaves;
   const int64_t k0 = wave_id() * each, k1 = k0 + each < count ? k0 + each : count;
   const int64_t unit = (blockIdx.x - chunk * g.segs) * kWave + lane_id();
   const int64_t c = unit * kPer<T>;
   float s[kPer<T>] = {};
   if (c < g.D) {
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t k = k0; k < k1; k++) {
       const float *from = chunk_sum<T>(part, g, chunk + k, k == 0 ? 1 : 0, unit);
 #pragma unroll
@@ -142,7 +147,138 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_join_kernel(TO *__restri
   for (int v = 1; v < kWaves; v++)
 #pragma unroll
     for (int i = 0; i < kPer<T>; i++) s[i] += sums[v][lane_id()][i];
-  store_sums<T, TO, ADD>(dE + (int64_t)run * g.ldE + c, s, g.D - c);
+  store_sums<T, TO, ADD, STREAM>(dE + (int64_t)run * g.ldE + c, s, g.D - c);
+}
+
+// ------------------------------------------------------------------------------------------------ few ids
+// Up to 256 ids in one launch, without a workspace.  The first `segs` workgroups take 64 pieces of the rows each: every
+// one of them orders the ids for itself (an id's place is how many are smaller, its place in the batch being the low byte
+// of what is compared; four threads share the counting for one id), its 16 waves sum a chunk each, and the runs that cross
+// chunks are joined through LDS.  The other workgroups zero those of their rows that no id names.  The same sums in the
+// same order every time.  For tables of fewer than 2^24 rows; beyond that the ordered path takes over.
+// What every lane of a wave has read, as the scalar that it is: a wave then branches instead of masking its lanes.
+__device__ __forceinline__ uint32_t one(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+
+constexpr int kFewIds = 256;
+constexpr int64_t kFewTable = ((int64_t)1 << 24) - 1;
+constexpr int kFewWaves = 16;
+constexpr int kFewFillRows = 2048;
+
+template <class T, class TO, class I, bool ADD, bool STREAM>
+__global__ __launch_bounds__(kFewWaves *kWave) void lookup_grad_few_kernel(TO *__restrict__ dE, const T *__restrict__ dy,
+                                                                           const I *__restrict__ ids, const float *__restrict__ vals,
+                                                                           float scale, GradShape g, int fill_rows) {
+  __shared__ __align__(16) uint32_t key[kFewIds];
+  __shared__ uint32_t okey[kFewIds];
+  __shared__ int oitem[kFewIds];
+  __shared__ float part[kFewWaves][2][kWave][kPer<T>];
+  const int n = (int)g.n, t = (int)threadIdx.x, lane = lane_id(), w = wave_id();
+  const uint32_t none = (uint32_t)g.V;
+
+  if ((int64_t)blockIdx.x >= g.segs) {
+    if (ADD) return;
+    uint8_t *named = (uint8_t *)&part[0][0][0][0];
+    const int64_t first = ((int64_t)blockIdx.x - g.segs) * fill_rows;
+    for (int r = t; r < fill_rows; r += kFewWaves * kWave) named[r] = 0;
+    __syncthreads();
+    if (t < n) {
+      const int64_t v = (int64_t)ids[t];
+      if (v >= first && v < g.V && v - first < fill_rows) named[v - first] = 1;
+    }
+    __syncthreads();
+    const int lanes = 1 << g.fill.lg, each = kWave >> g.fill.lg;
+    const Piece<TO> z = {};
+    for (int r0 = w * each; r0 < fill_rows; r0 += kFewWaves * each) {
+      const int r = r0 + lane / lanes;
+      if (r >= fill_rows || first + r >= g.V || named[r]) continue;
+      TO *row = dE + (first + r) * g.ldE;
+      for (int64_t c = (int64_t)(lane & (lanes - 1)) * kPer<TO>; c < g.D; c += (int64_t)lanes * kPer<TO>) store_piece<STREAM>(row + c, z, g.D - c);
+    }
+    return;
+  }
+
+  if (t < kFewIds) {
+    const int64_t v = t < n ? (int64_t)ids[t] : -1;
+    key[t] = (v >= 0 && v < g.V ? (uint32_t)v : none) << 8 | (uint32_t)t;
+  }
+  __syncthreads();
+  {
+    const uint32_t mine = key[t >> 2];
+    const int quarter = (n + 15) / 16 * 4;  // whole reads of four; what lies behind the n-th is larger than all before it
+    int before = 0;
+    for (int u = (t & 3) * quarter; u < ((t & 3) + 1) * quarter; u += 4) {
+      const uint4 k = *(const uint4 *)&key[u];
+      before += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
+    }
+    before += __shfl_xor(before, 1, kWave);
+    before += __shfl_xor(before, 2, kWave);
+    if ((t & 3) == 0 && (t >> 2) < n) {
+      okey[before] = mine >> 8;
+      oitem[before] = (int)(mine & 255);
+    }
+  }
+  __syncthreads();
+
+  const int64_t c = ((int64_t)blockIdx.x * kWave + lane) * kPer<T>;
+  const int chunk = (n + kFewWaves - 1) / kFewWaves;
+  const int p0 = w * chunk, p1 = p0 + chunk < n ? p0 + chunk : n;
+  if (p0 < p1) {
+    constexpr int R = 8;
+    uint32_t run = one(okey[p0]);
+    bool from_before = p0 > 0 && one(okey[p0 - 1]) == run;
+    float s[kPer<T>] = {};
+    for (int p = p0; p < p1 && run != none; p += R) {
+      uint32_t k[R];
+      float f[R];
+      Piece<T> x[R];
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        k[r] = p + r < p1 ? one(okey[p + r]) : none;
+        const int i = k[r] != none ? (int)one(oitem[p + r]) : 0;
+        f[r] = vals ? scale * vals[i] : scale;
+        x[r] = load_piece(dy + (int64_t)i * g.ldy + c, k[r] != none ? g.D - c : 0);
+      }
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        if (k[r] != run) {
+          if (p + r >= p1) break;
+          if (from_before) {
+#pragma unroll
+            for (int i = 0; i < kPer<T>; i++) part[w][0][lane][i] = s[i];
+          } else if (c < g.D) {
+            store_sums<T, TO, ADD, STREAM>(dE + (int64_t)run * g.ldE + c, s, g.D - c);
+          }
+          run = k[r];
+          from_before = false;
+#pragma unroll
+          for (int i = 0; i < kPer<T>; i++) s[i] = 0.0f;
+          if (run == none) break;
+        }
+#pragma unroll
+        for (int i = 0; i < kPer<T>; i++) s[i] += f[r] * (float)x[r].v[i];
+      }
+    }
+    if (run != none) {
+      const bool goes_on = p1 < n && one(okey[p1]) == run;
+      if (from_before || goes_on) {
+#pragma unroll
+        for (int i = 0; i < kPer<T>; i++) part[w][from_before ? 0 : 1][lane][i] = s[i];
+      } else if (c < g.D) {
+        store_sums<T, TO, ADD, STREAM>(dE + (int64_t)run * g.ldE + c, s, g.D - c);
+      }
+    }
+  }
+  __syncthreads();
+  if (p0 >= p1 || p1 >= n) return;
+  const uint32_t run = one(okey[p1 - 1]);
+  if (run == none || one(okey[p1]) != run || (p0 > 0 && one(okey[p0 - 1]) == run)) return;
+  float s[kPer<T>];
+#pragma unroll
+  for (int i = 0; i < kPer<T>; i++) s[i] = part[w][1][lane][i];
+  for (int v = w + 1; v * chunk < n && one(okey[v * chunk]) == run; v++)
+#pragma unroll
+    for (int i = 0; i < kPer<T>; i++) s[i] += part[v][0][lane][i];
+  if (c < g.D) store_sums<T, TO, ADD, STREAM>(dE + (int64_t)run * g.ldE + c, s, g.D - c);
 }
 
 }  // namespace tok

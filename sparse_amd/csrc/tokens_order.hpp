@@ -3,10 +3,12 @@
 //
 // A pass ranks each item among the equal digits of its wave (one ballot per digit bit), counts the waves' digits in LDS,
 // and turns the counts into places by one scan; nothing is ordered by an atomic, so equal inputs give equal orders.
-// Up to 8192 items one workgroup does everything in a single launch.  Beyond that the items are split over at most 256
+// Few items (4096 choices, 2048 ids) are ordered by one workgroup in a single launch.  More are split over at most 128
 // workgroups: one launch counts every workgroup's digits, the next adds up the counts of the workgroups before its own
-// (a column of at most 256 numbers per bin, out of L2) and places its items.  Items are 4 to 16 bytes each against rows
-// of hundreds or thousands, so these launches are bound by their latency, and there are few of them for that reason.
+// (a column of at most 128 numbers per bin, out of L2) and places its items.  Items are 4 to 16 bytes each against rows
+// of hundreds or thousands, so these launches are bound by their latency and by the ballots of the ranks: a wave ranks
+// only 64 items at a time where there are workgroups enough (16384 ids of 18 bits: 17 us in four launches; with two items
+// a lane 27 us, by one workgroup 43 us).
 #pragma once
 
 #include "tokens_common.hpp"
@@ -16,9 +18,10 @@ namespace tok {
 
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxBins = kMaxExperts + 1;  // the last bin: choices that name no expert
-constexpr int kOneGroup = 8192;            // items one workgroup orders by itself
-constexpr int kTile = 2048;                // items a workgroup of a split pass places at a time
-constexpr int kMaxGroups = 256;
+constexpr int kOneGroupChoices = 4096, kOneGroupIds = 2048;  // what one workgroup orders by itself
+constexpr int kSplitWaves = 8, kSplitThreads = kSplitWaves * kWave;
+constexpr int kTile = kSplitThreads;       // items a workgroup of a split pass places at a time
+constexpr int kMaxGroups = 128;
 
 // Rank of every item among the items of its wave with the same digit that come before it.  The wave's items are
 // first + i * 64 + lane; digit < 0: no item.  cnt[d] (this wave's own, zeroed by the caller) ends as the wave's counts.
@@ -143,19 +146,19 @@ struct Digits {
   __device__ __forceinline__ int digit(uint32_t k) const { return BY == 0 ? (int)k : (int)((k >> shift) & (uint32_t)mask); }
 };
 
-// hist[g * bins + b] = how many of workgroup g's items have digit b.  `clear`: words to zero on the way (the next pass's
-// counts, the marks of the ids that occur), each workgroup its share.
+// hist[g * bins + b] = how many of workgroup g's items have digit b.  `clear`: null, or words to zero on the way.
 template <int BY, class I>
-__global__ __launch_bounds__(kThreads) void digit_count_kernel(Digits<BY, I> d, int64_t per_group, int bins, int *__restrict__ hist,
-                                                               uint32_t *__restrict__ clear, int64_t clear_words) {
+__global__ __launch_bounds__(kSplitThreads) void digit_count_kernel(Digits<BY, I> d, int64_t per_group, int bins, int *__restrict__ hist,
+                                                                    uint32_t *__restrict__ clear, int64_t clear_words) {
   __shared__ int cnt[kMaxBins];
-  for (int b = threadIdx.x; b < bins; b += kThreads) cnt[b] = 0;
+  for (int64_t k = (int64_t)blockIdx.x * kSplitThreads + threadIdx.x; k < clear_words; k += (int64_t)gridDim.x * kSplitThreads) clear[k] = 0;
+  for (int b = threadIdx.x; b < bins; b += kSplitThreads) cnt[b] = 0;
   __syncthreads();
   const int64_t i0 = (int64_t)blockIdx.x * per_group, i1 = i0 + per_group < d.n ? i0 + per_group : d.n;
-  for (int64_t i = i0 + threadIdx.x; i < i1; i += kThreads) atomicAdd(&cnt[d.digit(d.key(i))], 1);
+#pragma unroll 2
+  for (int64_t i = i0 + threadIdx.x; i < i1; i += kSplitThreads) atomicAdd(&cnt[d.digit(d.key(i))], 1);
   __syncthreads();
-  for (int b = threadIdx.x; b < bins; b += kThreads) hist[(int64_t)blockIdx.x * bins + b] = cnt[b];
-  for (int64_t k = (int64_t)blockIdx.x * kThreads + threadIdx.x; k < clear_words; k += (int64_t)gridDim.x * kThreads) clear[k] = 0;
+  for (int b = threadIdx.x; b < bins; b += kSplitThreads) hist[(int64_t)blockIdx.x * bins + b] = cnt[b];
 }
 
 struct PassOut {
@@ -163,28 +166,26 @@ struct PassOut {
   uint32_t *keys;                    // ids: the keys and the items in their new order
   int32_t *items;
   const int32_t *items_in;           // null: item i is i
-  int *next_hist;                    // null: no further pass; else its counts (zeroed), by the workgroup of the new place
-  int next_shift, next_mask, next_bins;
-  uint32_t *marks;                   // null, or one bit for every row of the table: set where an id names it
+  uint8_t *named;                    // null, or a byte for every row of the table (zeroed): set where an id names it
 };
 
 template <int BY, class I>
-__global__ __launch_bounds__(kThreads) void digit_place_kernel(Digits<BY, I> d, int64_t per_group, int bins, int bits,
-                                                               const int *__restrict__ hist, PassOut o) {
-  constexpr int IPL = kTile / kThreads;
-  __shared__ int cnt[kWaves * kMaxBins];
+__global__ __launch_bounds__(kSplitThreads) void digit_place_kernel(Digits<BY, I> d, int64_t per_group, int bins, int bits,
+                                                                    const int *__restrict__ hist, PassOut o) {
+  constexpr int IPL = kTile / kSplitThreads;
+  __shared__ int cnt[kSplitWaves * kMaxBins];
   __shared__ int base[kMaxBins];
-  __shared__ int wave_total[kWaves];
+  __shared__ int wave_total[kSplitWaves];
   const int groups = (int)gridDim.x, g = (int)blockIdx.x;
   const int64_t i0 = (int64_t)g * per_group, i1 = i0 + per_group < d.n ? i0 + per_group : d.n;
 
   // base[b] = items with a smaller digit, and those with digit b in workgroups before this one
-  const int per = (bins + kThreads - 1) / kThreads;
+  const int per = (bins + kSplitThreads - 1) / kSplitThreads;
   const int b0 = (int)threadIdx.x * per, b1 = min(b0 + per, bins);
   int all = 0;
   for (int b = b0; b < b1; b++) {
     int before = 0, total = 0;
-#pragma unroll 8
+#pragma unroll 16
     for (int k = 0; k < groups; k++) {
       const int c = hist[(int64_t)k * bins + b];
       total += c;
@@ -195,7 +196,7 @@ __global__ __launch_bounds__(kThreads) void digit_place_kernel(Digits<BY, I> d, 
     all += total;
   }
   int unused;
-  int at = group_scan<kWaves>(all, wave_total, &unused);
+  int at = group_scan<kSplitWaves>(all, wave_total, &unused);
   for (int b = b0; b < b1; b++) {
     if (BY == 0 && g == 0) o.offsets[b] = at;
     base[b] += at;
@@ -204,8 +205,6 @@ __global__ __launch_bounds__(kThreads) void digit_place_kernel(Digits<BY, I> d, 
   __syncthreads();
 
   for (int64_t t0 = i0; t0 < i1; t0 += kTile) {
-    for (int b = threadIdx.x; b < kWaves * bins; b += kThreads) cnt[b] = 0;
-    __syncthreads();
     const int64_t first = t0 + wave_id() * (kWave * IPL) + lane_id();
     uint32_t key[IPL];
     int digit[IPL], rank[IPL];
@@ -215,13 +214,15 @@ __global__ __launch_bounds__(kThreads) void digit_place_kernel(Digits<BY, I> d, 
       key[i] = at_i < i1 ? d.key(at_i) : 0u;
       digit[i] = at_i < i1 ? d.digit(key[i]) : -1;
     }
+    for (int b = threadIdx.x; b < kSplitWaves * bins; b += kSplitThreads) cnt[b] = 0;
+    __syncthreads();
     int *mine = cnt + wave_id() * bins;
     wave_ranks<IPL>(digit, rank, bits, mine);
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += kThreads) {
+    for (int b = threadIdx.x; b < bins; b += kSplitThreads) {
       int run = base[b];
 #pragma unroll
-      for (int w = 0; w < kWaves; w++) {
+      for (int w = 0; w < kSplitWaves; w++) {
         const int c = cnt[w * bins + b];
         cnt[w * bins + b] = run;
         run += c;
@@ -239,8 +240,7 @@ __global__ __launch_bounds__(kThreads) void digit_place_kernel(Digits<BY, I> d, 
       } else {
         o.keys[place] = key[i];
         o.items[place] = o.items_in ? o.items_in[at_i] : (int32_t)at_i;
-        if (o.next_hist) atomicAdd(&o.next_hist[(place / per_group) * o.next_bins + ((key[i] >> o.next_shift) & (uint32_t)o.next_mask)], 1);
-        if (o.marks && (int64_t)key[i] < d.V) atomicOr(&o.marks[key[i] >> 5], 1u << (key[i] & 31));
+        if (o.named && (int64_t)key[i] < d.V) o.named[key[i]] = 1;
       }
     }
     __syncthreads();
@@ -248,20 +248,20 @@ __global__ __launch_bounds__(kThreads) void digit_place_kernel(Digits<BY, I> d, 
 }
 
 // ------------------------------------------------------------------------------------------------ ids by table row, small
-// All passes of up to 8192 ids in one workgroup, keys and items in LDS between them.
+// All passes of up to 2048 ids in one workgroup, keys and items in LDS between them.
 constexpr int kSmallBits = 9;
 
 template <class I, int IPL>
 __global__ __launch_bounds__(1024) void id_sort_small_kernel(const I *__restrict__ ids, int n, int64_t V, int passes, int bits,
                                                              uint32_t *__restrict__ keys, int32_t *__restrict__ items,
-                                                             uint32_t *__restrict__ marks, int64_t mark_words) {
+                                                             uint8_t *__restrict__ named) {
   constexpr int NW = 16;
   __shared__ uint32_t skey[NW * kWave * IPL];
-  __shared__ int32_t sitem[NW * kWave * IPL];
+  __shared__ uint16_t sitem[NW * kWave * IPL];
   __shared__ int cnt[NW << kSmallBits];
   __shared__ int wave_total[NW];
-  if (marks) {
-    for (int64_t k = threadIdx.x; k < mark_words; k += NW * kWave) marks[k] = 0;
+  if (named) {  // a byte for every row of the table, a whole number of words
+    for (int64_t k = threadIdx.x; k < (V + 3) / 4; k += NW * kWave) ((uint32_t *)named)[k] = 0;
     __syncthreads();
   }
   const int first = wave_id() * kWave * IPL + lane_id();
@@ -276,9 +276,8 @@ __global__ __launch_bounds__(1024) void id_sort_small_kernel(const I *__restrict
     item[i] = at;
     if (at < n) {
       const int64_t v = (int64_t)ids[at];
-      const bool in = v >= 0 && v < V;
-      key[i] = (uint32_t)(in ? v : V);
-      if (marks && in) atomicOr(&marks[key[i] >> 5], 1u << (key[i] & 31));
+      key[i] = (uint32_t)(v >= 0 && v < V ? v : V);
+      if (named && (int64_t)key[i] < V) named[key[i]] = 1;
     }
   }
   for (int p = 0; p < passes; p++) {
@@ -299,7 +298,7 @@ __global__ __launch_bounds__(1024) void id_sort_small_kernel(const I *__restrict
           items[place] = item[i];
         } else {
           skey[place] = key[i];
-          sitem[place] = item[i];
+          sitem[place] = (uint16_t)item[i];
         }
       }
     __syncthreads();

@@ -6,7 +6,8 @@
 //   combine       y[t]  = sum_j (w[t,j]) ys[pos[t,j]]     and back; the transpose of dispatch with the same places and weights
 //   combine_grad  dys[pos[t,j]] = w[t,j] dy[t],  dw[t,j] = <dy[t], ys[pos[t,j]]>
 //
-// All of them are bound by the bytes of the rows: every row is read once (dispatch reads a token's row once for all its
+// All of them are bound by the bytes of the rows (16384 tokens of 2048 bf16 to 8 places each: 604 MB, dispatch 121 us,
+// combine 106 us; with ordinary loads and stores instead of streaming ones 172 and 160 us): every row is read once (dispatch reads a token's row once for all its
 // places, combine_grad reads dy once for both of its results), nothing is held in memory between, sums are in 32 bits and
 // are rounded once, in an order that depends on the record alone.
 #pragma once
@@ -18,11 +19,11 @@ namespace tok {
 
 // ids outside 0 .. V-1 select nothing: a row of zeros (padding).
 // One wave takes U x 64 pieces of a row: U independent 16-byte loads in flight for each lane, behind one id.
-template <class T, class I, int U>
+template <class T, class I, int U, bool STREAM>
 __global__ __launch_bounds__(kThreads) void lookup_kernel(T *__restrict__ y, int64_t ldy, const T *__restrict__ E, int64_t ldE,
                                                           int64_t V, int64_t D, const I *__restrict__ ids, int64_t n,
                                                           const float *__restrict__ vals, float scale, int lg, int64_t segs) {
-  const RowPlace at = my_row(lg, segs, U);
+  const RowPlace at = my_row(wave_number(), lg, segs, U);
   if (at.row >= n) return;
   const int64_t id = (int64_t)ids[at.row];
   const bool any = id >= 0 && id < V;
@@ -43,7 +44,7 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(T *__restrict__ y, int
     if (!copy && any)
 #pragma unroll
       for (int i = 0; i < kPer<T>; i++) p[u].v[i] = (T)(f * (float)p[u].v[i]);
-    store_piece(dst + c, p[u], D - c);
+    store_piece<STREAM>(dst + c, p[u], D - c);
   }
 }
 
@@ -67,18 +68,18 @@ __global__ __launch_bounds__(kThreads) void lookup_dots_kernel(float *__restrict
 }
 
 // pos < 0: the token has no such place.  A place is given to one (t, j) only, so no two waves write one row.
-template <class T, int U>
+template <class T, int U, bool STREAM>
 __global__ __launch_bounds__(kThreads) void dispatch_kernel(T *__restrict__ xs, int64_t ldxs, const T *__restrict__ x, int64_t ldx,
                                                             int64_t n, int64_t D, int K, const int32_t *__restrict__ pos,
                                                             int64_t slots, const float *__restrict__ w, int lg, int64_t segs) {
-  const RowPlace at = my_row(lg, segs, U);
+  const RowPlace at = my_row(wave_number(), lg, segs, U);
   if (at.row >= n) return;
   const T *src = x + at.row * ldx;
   Piece<T> p[U];
 #pragma unroll
   for (int u = 0; u < U; u++) {
     const int64_t c = (at.unit + u * kWave) * kPer<T>;
-    p[u] = load_piece(src + c, D - c);
+    p[u] = load_piece<true>(src + c, D - c);
   }
   for (int j = 0; j < K; j++) {
     const int64_t to = pos[at.row * K + j];
@@ -92,18 +93,18 @@ __global__ __launch_bounds__(kThreads) void dispatch_kernel(T *__restrict__ xs, 
       if (w)
 #pragma unroll
         for (int i = 0; i < kPer<T>; i++) q.v[i] = (T)(f * (float)q.v[i]);
-      store_piece(xs + to * ldxs + c, q, D - c);
+      store_piece<STREAM>(xs + to * ldxs + c, q, D - c);
     }
   }
 }
 
 // The places of four choices at once: their rows are loaded before the first is added.
-template <class T, int U>
+template <class T, int U, bool STREAM>
 __global__ __launch_bounds__(kThreads) void combine_kernel(T *__restrict__ y, int64_t ldy, const T *__restrict__ ys, int64_t ldys,
                                                            int64_t n, int64_t D, int K, const int32_t *__restrict__ pos,
                                                            int64_t slots, const float *__restrict__ w, int lg, int64_t segs) {
   constexpr int J = 4;
-  const RowPlace at = my_row(lg, segs, U);
+  const RowPlace at = my_row(wave_number(), lg, segs, U);
   if (at.row >= n) return;
   float s[U][kPer<T>] = {};
   for (int j0 = 0; j0 < K; j0 += J) {
@@ -122,7 +123,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(T *__restrict__ y, in
 #pragma unroll
       for (int u = 0; u < U; u++) {
         const int64_t c = (at.unit + u * kWave) * kPer<T>;
-        p[j][u] = load_piece(ys + (from[j] < 0 ? 0 : from[j]) * ldys + c, from[j] < 0 ? 0 : D - c);
+        p[j][u] = load_piece<true>(ys + (from[j] < 0 ? 0 : from[j]) * ldys + c, from[j] < 0 ? 0 : D - c);
       }
 #pragma unroll
     for (int j = 0; j < J; j++)
@@ -135,13 +136,13 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(T *__restrict__ y, in
 #pragma unroll
   for (int u = 0; u < U; u++) {
     const int64_t c = (at.unit + u * kWave) * kPer<T>;
-    if (c < D) store_sums<T, T, false>(y + at.row * ldy + c, s[u], D - c);
+    if (c < D) store_sums<T, T, false, STREAM>(y + at.row * ldy + c, s[u], D - c);
   }
 }
 
 // One workgroup per token, its waves side by side along the row; eight choices at once share one reading of dy.  The dot
 // products are summed lane, wave, workgroup: the same order every time.
-template <class T>
+template <class T, bool STREAM>
 __global__ __launch_bounds__(kThreads) void combine_grad_kernel(T *__restrict__ dys, int64_t lddys, float *__restrict__ dw,
                                                                 const T *__restrict__ dy, int64_t lddy, const T *__restrict__ ys,
                                                                 int64_t ldys, int64_t D, int K, const int32_t *__restrict__ pos,
@@ -161,11 +162,11 @@ __global__ __launch_bounds__(kThreads) void combine_grad_kernel(T *__restrict__ 
       dot[j] = 0.0f;
     }
     for (int64_t c = (int64_t)threadIdx.x * kPer<T>; c < D; c += kThreads * kPer<T>) {
-      const Piece<T> g = load_piece(dy + t * lddy + c, D - c);
+      const Piece<T> g = load_piece<true>(dy + t * lddy + c, D - c);
       Piece<T> p[J];
 #pragma unroll
       for (int j = 0; j < J; j++)
-        if (at[j] >= 0) p[j] = load_piece(ys + at[j] * ldys + c, D - c);
+        if (at[j] >= 0) p[j] = load_piece<true>(ys + at[j] * ldys + c, D - c);
 #pragma unroll
       for (int j = 0; j < J; j++) {
         if (at[j] < 0) continue;
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(kThreads) void combine_grad_kernel(T *__restrict__ 
           dot[j] += (float)g.v[i] * (float)p[j].v[i];
           q.v[i] = (T)(f[j] * (float)g.v[i]);
         }
-        store_piece(dys + at[j] * lddys + c, q, D - c);
+        store_piece<STREAM>(dys + at[j] * lddys + c, q, D - c);
       }
     }
 #pragma unroll

@@ -58,12 +58,24 @@ _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream
 class Routing:
     """Where a batch's choices go (tk.route).  pos[tokens, K]: the place of every choice, -1 where it names no expert;
     src[tokens * K]: the choice (token * K + j) at every place, -1 behind the last; offsets[X + 1]: expert e has the places
-    offsets[e] .. offsets[e + 1] - 1.  All int32, on the device."""
-    __slots__ = ("pos", "src", "offsets", "tokens", "K", "X", "slots")
+    offsets[e] .. offsets[e + 1] - 1.  All int32, on the device, in one buffer."""
+    __slots__ = ("tokens", "K", "X", "slots", "_buf", "_pos", "_offsets")
 
-    def __init__(self, pos, src, offsets, tokens, K, X):
-        self.pos, self.src, self.offsets = pos, src, offsets
+    def __init__(self, buf, address, tokens, K, X):
         self.tokens, self.K, self.X, self.slots = tokens, K, X, tokens * K
+        self._buf, self._pos, self._offsets = buf, address, address + 8 * tokens * K
+
+    @property
+    def pos(self):
+        return self._buf[:self.slots].view(self.tokens, self.K)
+
+    @property
+    def src(self):
+        return self._buf[self.slots:2 * self.slots]
+
+    @property
+    def offsets(self):
+        return self._buf[2 * self.slots:]
 
 
 class mk_tokens:
@@ -75,6 +87,7 @@ class mk_tokens:
         self._code, self._dtype = _TYPES[T]
         self.ctx = ctx if ctx is not None else default_context()
         self._dev = self.ctx.device
+        self._device = torch.device("cuda", self._dev)
         L = self.ctx.L
         for name, types in _SIGNATURES.items():
             f = getattr(L, "sparse_amd_tokens_" + name)
@@ -110,7 +123,7 @@ class mk_tokens:
     def _flat(self, a, name, dtypes, shape=None):
         """Address of a contiguous tensor (of that shape)."""
         p = self._tensor(a, name, dtypes, None)
-        if shape is not None and tuple(a.shape) != tuple(shape):
+        if shape is not None and a.shape != shape:
             raise SparseError("%s: expected shape %s, got %s" % (name, tuple(shape), tuple(a.shape)))
         if not a.is_contiguous():
             raise SparseError("%s: not contiguous" % name)
@@ -124,7 +137,7 @@ class mk_tokens:
         """The result's panel: `out`, checked, or a new one."""
         dtype = dtype or self._dtype
         if out is None:
-            out = torch.empty((rows, cols), dtype=dtype, device=torch.device("cuda", self._dev))
+            out = torch.empty((rows, cols), dtype=dtype, device=self._device)
             return out, out.data_ptr(), max(cols, 1)
         p, ld, _, _ = self._panel(out, name, rows, cols, (dtype,))
         return out, p, ld
@@ -144,7 +157,7 @@ class mk_tokens:
         being captured."""
         if size == 0:
             return None, None
-        w = torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", self._dev))
+        w = torch.empty(size, dtype=torch.uint8, device=self._device)
         return w, w.data_ptr()
 
     # ---- one entry per row
@@ -195,12 +208,13 @@ class mk_tokens:
             raise SparseError("chosen: expected 2 dimensions, got %d" % chosen.dim())
         c, bits, n = self._ids(chosen, "chosen")
         X = int(X)
-        buf = torch.empty(2 * n + max(X, 0) + 1, dtype=torch.int32, device=chosen.device)
+        buf = torch.empty(2 * n + max(X, 0) + 1, dtype=torch.int32, device=self._device)
         size = self._c_route_work(n, X)
         w, wp = self._scratch(size)
         p = buf.data_ptr()
         self._call(self._c_route, c, bits, n, X, p, p + 4 * n, p + 8 * n, wp, size)
-        return Routing(buf[:n].view(chosen.shape), buf[n:2 * n], buf[2 * n:], chosen.shape[0], chosen.shape[1], X)
+        tokens, K = chosen.shape
+        return Routing(buf, p, tokens, K, X)
 
     def _routing(self, r):
         if not isinstance(r, Routing):
@@ -210,15 +224,12 @@ class mk_tokens:
     def _weights(self, w, r):
         return self._flat(w, "weights", (torch.float32,), (r.tokens, r.K)) if w is not None else None
 
-    def _pos(self, r):
-        return self._flat(r.pos, "pos", (torch.int32,), (r.tokens, r.K))
-
     def dispatch(self, x, r, weights=None, out=None):
         """xs[pos[t, j]] = weights[t, j] * x[t]: [slots, D], rows in the order of their experts."""
         r = self._routing(r)
         a, lda, n, D = self._panel(x, "x", rows=r.tokens)
         xs, p, ld = self._out(out, "out", r.slots, D)
-        self._call(self._c_dispatch, self._code, p, ld, r.slots, a, lda, n, D, r.K, self._pos(r), self._weights(weights, r))
+        self._call(self._c_dispatch, self._code, p, ld, r.slots, a, lda, n, D, r.K, r._pos, self._weights(weights, r))
         return xs
 
     def combine(self, ys, r, weights=None, out=None):
@@ -226,7 +237,7 @@ class mk_tokens:
         r = self._routing(r)
         a, lda, _, D = self._panel(ys, "ys", rows=r.slots)
         y, p, ld = self._out(out, "out", r.tokens, D)
-        self._call(self._c_combine, self._code, p, ld, a, lda, r.slots, r.tokens, D, r.K, self._pos(r), self._weights(weights, r))
+        self._call(self._c_combine, self._code, p, ld, a, lda, r.slots, r.tokens, D, r.K, r._pos, self._weights(weights, r))
         return y
 
     def dispatch_grad(self, dxs, r, weights=None, out=None):
@@ -243,8 +254,8 @@ class mk_tokens:
             raise SparseError("combine_grad: no weights (their absence makes the gradient dispatch(dy, r))")
         w = self._weights(weights, r)
         dys, p, ld = self._out(out, "out", r.slots, D)
-        dw = torch.empty((r.tokens, r.K), dtype=torch.float32, device=torch.device("cuda", self._dev))
-        self._call(self._c_combine_grad, self._code, p, ld, dw.data_ptr(), g, ldg, a, lda, r.slots, n, D, r.K, self._pos(r), w)
+        dw = torch.empty((r.tokens, r.K), dtype=torch.float32, device=self._device)
+        self._call(self._c_combine_grad, self._code, p, ld, dw.data_ptr(), g, ldg, a, lda, r.slots, n, D, r.K, r._pos, w)
         return dys, dw
 
     # ---- one dense block per expert
@@ -259,16 +270,13 @@ class mk_tokens:
             raise SparseError("%s: the elements of a row are not side by side" % name)
         return p, F, D, ld if F > 1 else max(ld, D), block
 
-    def _offsets(self, r):
-        return self._flat(r.offsets, "offsets", (torch.int32,), (r.X + 1,))
-
     def experts(self, xs, W, r, out=None):
         """ys[p] = W[e] xs[p] for every expert e's places p: [slots, F] from xs[slots, D], W[X, F, D]."""
         r = self._routing(r)
         w, F, D, ldw, block = self._blocks(W, "W", r.X)
         a, lda, n, _ = self._panel(xs, "xs", rows=r.slots, cols=D)
         ys, p, ld = self._out(out, "out", n, F)
-        self._call(self._c_experts, self._code, p, ld, a, lda, n, w, r.X, F, D, ldw, block, self._offsets(r))
+        self._call(self._c_experts, self._code, p, ld, a, lda, n, w, r.X, F, D, ldw, block, r._offsets)
         return ys
 
     def experts_grad_x(self, dys, W, r, out=None):
@@ -277,7 +285,7 @@ class mk_tokens:
         w, F, D, ldw, block = self._blocks(W, "W", r.X)
         a, lda, n, _ = self._panel(dys, "dys", rows=r.slots, cols=F)
         dxs, p, ld = self._out(out, "out", n, D)
-        self._call(self._c_experts_grad_x, self._code, p, ld, a, lda, n, w, r.X, F, D, ldw, block, self._offsets(r))
+        self._call(self._c_experts_grad_x, self._code, p, ld, a, lda, n, w, r.X, F, D, ldw, block, r._offsets)
         return dxs
 
     def experts_grad_w(self, dys, xs, r, out=None, accumulate=False, dtype=None):
@@ -290,9 +298,9 @@ class mk_tokens:
             raise SparseError("experts_grad_w: accumulate needs `out`")
         dtype, code = self._sum_type(out, dtype)
         if out is None:
-            out = torch.empty((r.X, F, D), dtype=dtype, device=torch.device("cuda", self._dev))
+            out = torch.empty((r.X, F, D), dtype=dtype, device=self._device)
         w, f, d, ldw, block = self._blocks(out, "out", r.X, (dtype,))
         if (f, d) != (F, D):
             raise SparseError("out: expected blocks of %d x %d, got %d x %d" % (F, D, f, d))
-        self._call(self._c_experts_grad_w, self._code, code, int(accumulate), w, r.X, F, D, ldw, block, g, ldg, a, lda, n, self._offsets(r))
+        self._call(self._c_experts_grad_w, self._code, code, int(accumulate), w, r.X, F, D, ldw, block, g, ldg, a, lda, n, r._offsets)
         return out

@@ -71,8 +71,8 @@ REFUSED = [
     (lookup, dict(ldy=63), "apart"), (lookup, dict(n=-1), "negative"), (lookup, dict(y=None), "null"), (lookup, dict(ids=None), "null"),
     (lookup, dict(table=None), "null"), (lookup, dict(y=B + 64), "overlaps"), (lookup, dict(y=C), "overlaps"), (lookup, dict(y=A + 1), "aligned"),
     (lookup, dict(vals=A + 8), "overlaps"), (lookup, dict(ids=C + 4), "aligned"), (lookup, dict(ldt=1 << 50), "too large"),
-    (grad, dict(out=F16), "32 bits"), (grad, dict(size=100), "workspace of"), (grad, dict(work=None), "workspace of"),
-    (grad, dict(work=W + 8), "aligned to 256"), (grad, dict(work=A), "overlaps"), (grad, dict(dt=B), "overlaps"), (grad, dict(V=1 << 31), "31 bits"),
+    (grad, dict(out=F16), "32 bits"), (grad, dict(n=300, size=100), "workspace of"), (grad, dict(n=300, work=None), "workspace of"),
+    (grad, dict(n=300, work=W + 8), "aligned to 256"), (grad, dict(work=A), "overlaps"), (grad, dict(dt=B), "overlaps"), (grad, dict(V=1 << 31), "31 bits"),
     (grad, dict(n=1 << 31), "31 bits"), (grad, dict(bits=8), "32 or 64 bits"),
     (route, dict(X=0), "experts"), (route, dict(X=1025), "experts"), (route, dict(n=-1), "negative"), (route, dict(n=1 << 31), "31 bits"),
     (route, dict(pos=A), "overlaps"), (route, dict(src=B), "overlaps"), (route, dict(n=100000, size=64), "workspace of"), (route, dict(offsets=None), "null"),
@@ -109,12 +109,12 @@ def test_workspaces():
     L = load_library()
     f = L.sparse_amd_tokens_lookup_grad_workspace
     f.argtypes, f.restype = (ctypes.c_int, I64, I64, I64), I64
-    assert f(BF16, 0, 100, 64) == 0 and f(BF16, 10, 100, 0) == 0 and f(BF16, -1, 100, 64) == 0
+    assert f(BF16, 256, 100, 64) == 0 and f(BF16, 257, 100, 64) > 0 and f(BF16, 10, 100, 0) == 0 and f(BF16, -1, 100, 64) == 0
     # keys and items at least, and two rows of 32-bit sums for every chunk
     assert f(BF16, 10000, 1000, 64) > 8 * 10000 + 2 * (10000 // 32) * 64 * 4
     g = L.sparse_amd_tokens_route_workspace
     g.argtypes, g.restype = (I64, I64), I64
-    assert g(8192, 1024) == 0 and g(8193, 1024) >= 4 * 1025 and g(1 << 30, 1024) <= 2 << 20
+    assert g(4096, 1024) == 0 and g(4097, 1024) >= 4 * 1025 and g(1 << 30, 1024) <= 2 << 20
 
 
 def test_the_python_side_refuses_what_is_not_on_the_device():
