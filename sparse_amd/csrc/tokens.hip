@@ -269,7 +269,7 @@ bool direct_to_lds(const T *p, int64_t ld) {
   return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && ld <= ((int64_t)1 << 20);
 }
 
-template <class T, class TO, int KIND, int BM, int BN, int DEPTH, int WM, int WN, bool ADD>
+template <class T, class TO, int KIND, int BM, int BN, int DEPTH, int WM, int WN, bool ADD, bool ONCE = false>
 int launch_experts(futhark_context *ctx, const char *who, hipStream_t stream, TO *C, const T *A, const T *B, const int32_t *offsets,
                    ProductShape g) {
   const int64_t n_tiles = cdiv(g.N, BN);
@@ -289,7 +289,7 @@ int launch_experts(futhark_context *ctx, const char *who, hipStream_t stream, TO
   if constexpr (DEPTH == 0)
     TOK_LAUNCH(ctx, (experts_any_kernel<T, TO, KIND, BM, BN, WM, WN, ADD>), blocks, WM * WN * kWave, stream, C, A, B, offsets, g);
   else
-    TOK_LAUNCH(ctx, (experts_kernel<T, TO, KIND, BM, BN, DEPTH, WM, WN, ADD>), blocks, WM * WN * kWave, stream, C, A, B, offsets, g);
+    TOK_LAUNCH(ctx, (experts_kernel<T, TO, KIND, BM, BN, DEPTH, WM, WN, ADD, ONCE>), blocks, WM * WN * kWave, stream, C, A, B, offsets, g);
   return 0;
 }
 
@@ -298,10 +298,35 @@ int experts_panels(futhark_context *ctx, const char *who, hipStream_t stream, T 
                    const ProductShape &g) {
   const bool fast = direct_to_lds(A, g.ldA) && g.K % 8 == 0 && direct_to_lds(B, g.ldB) && g.blockB % 8 == 0;
   if (!fast) return launch_experts<T, T, KIND, 128, 128, 0, 2, 2, false>(ctx, who, stream, C, A, B, offsets, g);
-  const int64_t mean = g.rows / g.X;
-  if (mean <= 32) return launch_experts<T, T, KIND, 32, 128, 64, 1, 4, false>(ctx, who, stream, C, A, B, offsets, g);
-  if (mean < 256) return launch_experts<T, T, KIND, 128, 128, 32, 2, 2, false>(ctx, who, stream, C, A, B, offsets, g);
-  return launch_experts<T, T, KIND, 256, 256, 32, 2, 4, false>(ctx, who, stream, C, A, B, offsets, g);
+  // The tile whose launch is estimated to end first: whole rounds of the card's 256 CUs, by the rate each tile reaches with
+  // the card full (TFLOP/s, measured on 32 experts of 4096 x 2048).  Small tiles waste fewer rows of a small expert, large
+  // ones read each operand less often: 64 rows an expert, forward: 64 x 256 136 us, 256 x 256 146; 256 rows: 244 and 180.
+  struct { int bm, bn, per_cu, rate; } const tiles[] = {{32, 64, 3, 400}, {64, 256, 2, 600}, {128, 128, 2, 800}, {128, 256, 1, 900}, {256, 256, 1, 1200}};
+  const int64_t used = g.rows < g.X ? g.rows : g.X, mean = cdiv(g.rows, used);
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < 5; i++) {
+    const int64_t count = used * cdiv(mean, tiles[i].bm) * cdiv(g.N, tiles[i].bn);
+    const double t = (double)cdiv(count, 256 * tiles[i].per_cu) * tiles[i].per_cu * tiles[i].bm * tiles[i].bn / tiles[i].rate;
+    if (i == 0 || t < least) {
+      best = i;
+      least = t;
+    }
+  }
+  // weights that the card's last cache (256 MiB) cannot hold until the next call are read past it where a block is read
+  // once: 32 blocks of 4096 x 2048, 110 -> 95 us; 8 of them, which it holds, 22 -> 31
+  const bool once = mean <= tiles[best].bm && used * g.blockB * (int64_t)sizeof(T) > ((int64_t)256 << 20);
+  switch (best) {
+    case 0:
+      return once ? launch_experts<T, T, KIND, 32, 64, 64, 1, 4, false, true>(ctx, who, stream, C, A, B, offsets, g)
+                  : launch_experts<T, T, KIND, 32, 64, 64, 1, 4, false>(ctx, who, stream, C, A, B, offsets, g);
+    case 1:
+      return once ? launch_experts<T, T, KIND, 64, 256, 32, 1, 4, false, true>(ctx, who, stream, C, A, B, offsets, g)
+                  : launch_experts<T, T, KIND, 64, 256, 32, 1, 4, false>(ctx, who, stream, C, A, B, offsets, g);
+    case 2: return launch_experts<T, T, KIND, 128, 128, 32, 2, 2, false>(ctx, who, stream, C, A, B, offsets, g);
+    case 3: return launch_experts<T, T, KIND, 128, 256, 32, 2, 4, false>(ctx, who, stream, C, A, B, offsets, g);
+    default: return launch_experts<T, T, KIND, 256, 256, 32, 2, 4, false>(ctx, who, stream, C, A, B, offsets, g);
+  }
 }
 
 template <class T, class TO, bool ADD>
@@ -309,7 +334,9 @@ int experts_weights(futhark_context *ctx, const char *who, hipStream_t stream, T
                     const ProductShape &g) {
   if (!(direct_to_lds(A, g.ldA) && direct_to_lds(B, g.ldB)))
     return launch_experts<T, TO, kGradW, 128, 128, 0, 2, 2, ADD>(ctx, who, stream, C, A, B, offsets, g);
-  return launch_experts<T, TO, kGradW, 256, 256, 32, 2, 4, ADD>(ctx, who, stream, C, A, B, offsets, g);
+  // as above: tiles enough for every CU to have a large one
+  if (g.X * cdiv(g.M, 256) * cdiv(g.N, 256) >= 256) return launch_experts<T, TO, kGradW, 256, 256, 32, 2, 4, ADD>(ctx, who, stream, C, A, B, offsets, g);
+  return launch_experts<T, TO, kGradW, 128, 128, 32, 2, 2, ADD>(ctx, who, stream, C, A, B, offsets, g);
 }
 
 int check_experts(futhark_context *ctx, const char *who, int64_t rows, int64_t X, int64_t F, int64_t D, const int32_t *offsets) {
@@ -533,6 +560,7 @@ int sparse_amd_tokens_experts(struct futhark_context *ctx, void *stream, int typ
       if (rows == 0 || F == 0) return 0;
       ProductShape g = {};
       g.rows = rows; g.N = F; g.K = D; g.ldA = ldx; g.ldB = ldw; g.ldC = ldy; g.blockB = blockw; g.X = (int)X;
+      g.stream = rows * F * 2 > kStreamBytes;
       return experts_panels<T, kForward>(ctx, who, (hipStream_t)stream, (T *)ys, (const T *)xs, (const T *)w, offsets, g);
     });
   });
@@ -553,6 +581,7 @@ int sparse_amd_tokens_experts_grad_x(struct futhark_context *ctx, void *stream, 
       if (rows == 0 || D == 0) return 0;
       ProductShape g = {};
       g.rows = rows; g.N = D; g.K = F; g.ldA = ldy; g.ldB = ldw; g.ldC = ldx; g.blockB = blockw; g.X = (int)X;
+      g.stream = rows * D * 2 > kStreamBytes;
       return experts_panels<T, kGradX>(ctx, who, (hipStream_t)stream, (T *)dxs, (const T *)dys, (const T *)w, offsets, g);
     });
   });
@@ -575,6 +604,7 @@ int sparse_amd_tokens_experts_grad_w(struct futhark_context *ctx, void *stream, 
       if (F == 0 || D == 0) return 0;
       ProductShape g = {};
       g.rows = rows; g.M = F; g.N = D; g.ldA = ldy; g.ldB = ldx; g.ldC = ldw; g.blockC = blockw; g.X = (int)X;
+      g.stream = X * F * D * 2 > kStreamBytes;
       const hipStream_t s = (hipStream_t)stream;
       if (out_type == type)
         return accumulate ? experts_weights<T, T, true>(ctx, who, s, (T *)dw, (const T *)dys, (const T *)xs, offsets, g)

@@ -20,6 +20,8 @@
 
 #include "tokens_common.hpp"
 
+#include <type_traits>
+
 namespace samd {
 namespace tok {
 
@@ -52,6 +54,7 @@ struct ProductShape {
   int64_t blockB;      // elements from one block of W to the next (kForward, kGradX)
   int64_t blockC;      // elements from one block of dW to the next (kGradW)
   int X;
+  bool stream;         // the result is written past the caches
   int m_tiles, n_tiles;  // kForward / kGradX: m_tiles = upper bound over all experts; kGradW: of one block
 };
 
@@ -83,7 +86,7 @@ struct Tile {
       constexpr int per = R / 8;
       const int k = at / per, q = at % per;
       *row = k;
-      *col = (((q >> 1) ^ spread(k)) << 4) + ((q & 1) << 3);
+      *col = (((q >> 1) ^ (spread(k) & (R / 16 - 1))) << 4) + ((q & 1) << 3);
     } else {
       constexpr int per = DEPTH / 8;
       const int r = at / per, q = at % per;
@@ -123,7 +126,8 @@ struct Tile {
     bound();
   }
 
-  // FAST: starts the loads of step `step` into lds.
+  // FAST: starts the loads of step `step` into lds.  ONCE: past the caches' order of use (non-temporal).
+  template <bool ONCE = false>
   __device__ __forceinline__ void start(T *lds, int step) {
     int row, col;
     source(0, threadIdx.x, &row, &col);  // the same columns in every load of a thread: NT / (DEPTH / 8) rows on, twist() repeats
@@ -133,7 +137,7 @@ struct Tile {
     char *to = (char *)lds + wave_id() * (kWave * 16);
 #pragma unroll
     for (int i = 0; i < kLoads; i++)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(bounds, (LdsVoid *)(to + i * NT * 16), 16, (int)(dead ? 0x80000000u : off[i]), at, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(bounds, (LdsVoid *)(to + i * NT * 16), 16, (int)(dead ? 0x80000000u : off[i]), at, 0, ONCE ? 2 : 0);
   }
 
   // Not FAST: the step at summed index k0 into registers, and from there into lds.
@@ -158,7 +162,7 @@ struct Tile {
     typename Mfma<T>::Frag f;
     if (STANDING) {
       const int q = (l & 15) >> 2;
-      const int u = (r0 >> 4) ^ (q | (((l >> 4) & 1) << 2));
+      const int u = (r0 >> 4) ^ ((q | (((l >> 4) & 1) << 2)) & (R / 16 - 1));
       const T *at = lds + (kk * 32 + (l >> 4) * 8 + q) * R + u * 16 + (l & 3) * 4;
       const Short4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4 *)at);
       const Short4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4 *)(at + 4 * R));
@@ -296,6 +300,7 @@ __device__ __forceinline__ bool place_product(TA &ta, TB &tb, TO *&out, int64_t 
   return true;
 }
 
+// Sums in 32 bits, or added to what is there: every lane writes the four neighbouring columns that it holds.
 template <class T, class TO, bool ADD, int BM, int BN, int WM, int WN, class Acc, int NI, int MI>
 __device__ __forceinline__ void store_product(TO *out, const Acc (&acc)[NI][MI], int64_t m0, int64_t n0, int64_t m_end, const ProductShape &g) {
   const int l = lane_id(), wm = wave_id() / WN, wn = wave_id() % WN;
@@ -307,6 +312,40 @@ __device__ __forceinline__ void store_product(TO *out, const Acc (&acc)[NI][MI],
     for (int j = 0; j < NI; j++) {
       const int64_t n = n0 + wn * (BN / WN) + j * 16 + (l >> 4) * 4;
       if (n < g.N) store_four<T, TO, ADD>(out + m * g.ldC + n, acc[j][i], g.N - n);
+    }
+  }
+}
+
+// Rounded to 16 bits: through `mine`, LDS that only this wave uses, so that a row leaves the wave in pieces of 16 bytes that
+// lie side by side (a wave's 64 columns are a cache line; written four columns a lane, blocks of 4096 x 2048 for few rows took
+// 214 us where this takes 100).  The pieces of a row are permuted by the row's number: the lanes that write the same
+// columns of 16 rows would all meet in a few banks.
+template <class T, int BM, int BN, int WM, int WN, class Acc, int NI, int MI>
+__device__ __forceinline__ void store_rounded(T *mine, T *out, const Acc (&acc)[NI][MI], int64_t m0, int64_t n0, int64_t m_end, const ProductShape &g) {
+  constexpr int TM = BM / WM, TN = BN / WN, per = TN / 8;  // pieces in a row of the wave's tile
+  const int l = lane_id();
+  m0 += wave_id() / WN * TM;
+  n0 += wave_id() % WN * TN;
+#pragma unroll
+  for (int i = 0; i < MI; i++)
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+      const int r = i * 16 + (l & 15), c = j * 2 + (l >> 5);
+      T v[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) v[k] = (T)acc[j][i][k];
+      __builtin_memcpy((char *)mine + (r * per + (c ^ (r & (per - 1)))) * 16 + ((l >> 4) & 1) * 8, v, 8);
+    }
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int q = 0; q < TM * per / kWave; q++) {
+    const int at = q * kWave + l, r = at / per, c = at % per;
+    Piece<T> v;
+    __builtin_memcpy(&v, (const char *)mine + (r * per + (c ^ (r & (per - 1)))) * 16, 16);
+    const int64_t m = m0 + r, n = n0 + c * 8;
+    if (m < m_end) {
+      if (g.stream) store_piece<true>(out + m * g.ldC + n, v, g.N - n);
+      else store_piece<false>(out + m * g.ldC + n, v, g.N - n);
     }
   }
 }
@@ -363,7 +402,13 @@ __global__ __launch_bounds__(WM *WN *kWave) void experts_any_kernel(TO *__restri
       tb.put(sb[at ^ 1]);
     }
   }
-  store_product<T, TO, ADD, BM, BN, WM, WN>(out, acc, m0, n0, m_end, g);
+  if constexpr (std::is_same<T, TO>::value && !ADD) {
+    static_assert(BM / WM * (BN / WN) * WM * WN <= 2 * BM * DEPTH, "every wave's part of the tile fits into A's two buffers");
+    __syncthreads();
+    store_rounded<T, BM, BN, WM, WN>(&sa[0][0] + wave_id() * (BM / WM * (BN / WN)), out, acc, m0, n0, m_end, g);
+  } else {
+    store_product<T, TO, ADD, BM, BN, WM, WN>(out, acc, m0, n0, m_end, g);
+  }
 }
 
 // Rows that begin on 16 bytes.  Four stages of LDS, each DEPTH of the summed index: a stage's loads are started three steps
@@ -376,7 +421,9 @@ __global__ __launch_bounds__(WM *WN *kWave) void experts_any_kernel(TO *__restri
 // With eight waves, two on each SIMD, waves 4 to 7 run one barrier behind waves 0 to 3 and every step has a second
 // barrier behind its products: while one wave of a SIMD feeds the matrix cores the other reads LDS, and they change places.
 // A stage is then read half a step later by the second four, still before the barrier behind which it is overwritten.
-template <class T, class TO, int KIND, int BM, int BN, int DEPTH, int WM, int WN, bool ADD>
+//
+// ONCE: B is read past the caches, for weights that no cache could hold anyway.
+template <class T, class TO, int KIND, int BM, int BN, int DEPTH, int WM, int WN, bool ADD, bool ONCE>
 __global__ __launch_bounds__(WM *WN *kWave) void experts_kernel(TO *__restrict__ C, const T *__restrict__ A, const T *__restrict__ B,
                                                                 const int32_t *__restrict__ offsets, ProductShape g) {
   constexpr int NT = WM * WN * kWave, S = 4, KK = DEPTH / 32;
@@ -409,7 +456,7 @@ __global__ __launch_bounds__(WM *WN *kWave) void experts_kernel(TO *__restrict__
     }
     __builtin_amdgcn_sched_barrier(0);
     ta.start(na, t + S - 1);
-    tb.start(nb, t + S - 1);
+    tb.template start<ONCE>(nb, t + S - 1);
     __builtin_amdgcn_sched_barrier(0);
     arrived<(S - 2) * L>();
     __builtin_amdgcn_sched_barrier(0);
@@ -429,11 +476,11 @@ __global__ __launch_bounds__(WM *WN *kWave) void experts_kernel(TO *__restrict__
   };
   if (summed > 0) {
     ta.start(a0, 0);
-    tb.start(b0, 0);
+    tb.template start<ONCE>(b0, 0);
     ta.start(a1, 1);
-    tb.start(b1, 1);
+    tb.template start<ONCE>(b1, 1);
     ta.start(a2, 2);
-    tb.start(b2, 2);
+    tb.template start<ONCE>(b2, 2);
     arrived<(S - 2) * L>();
     const bool second = kPairs && wave_id() >= 4;
     if (second) __builtin_amdgcn_s_barrier();
@@ -448,7 +495,23 @@ __global__ __launch_bounds__(WM *WN *kWave) void experts_kernel(TO *__restrict__
     if (kPairs && !second) __builtin_amdgcn_s_barrier();  // as many barriers as the others
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // no load may still write to LDS when the workgroup has ended
   }
-  store_product<T, TO, ADD, BM, BN, WM, WN>(out, acc, m0, n0, m_end, g);
+  if constexpr (std::is_same<T, TO>::value && !ADD) {
+    constexpr int part = BM / WM * (BN / WN);  // each wave has a stage's array to itself, one that its part of the tile fits into
+    constexpr bool in_a = part <= BM * DEPTH;
+    static_assert(part <= BN * DEPTH && (in_a || !kPairs), "a wave's part of the tile fits into a stage's array");
+    __syncthreads();
+    T *const as[4] = {a0, a1, a2, a3}, *const bs[4] = {b0, b1, b2, b3};
+    const int w = wave_id();
+    T *mine = bs[0];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      if (w == k) mine = in_a ? as[k] : bs[k];
+      if (w == k + 4) mine = bs[k];
+    }
+    store_rounded<T, BM, BN, WM, WN>(mine, out, acc, m0, n0, m_end, g);
+  } else {
+    store_product<T, TO, ADD, BM, BN, WM, WN>(out, acc, m0, n0, m_end, g);
+  }
 }
 
 }  // namespace tok
