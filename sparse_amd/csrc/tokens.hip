@@ -283,6 +283,11 @@ int launch_experts(futhark_context *ctx, const char *who, hipStream_t stream, TO
     blocks = m_tiles * n_tiles;
   }
   blocks = cdiv(blocks, kXcds) * kXcds;
+  g.split = 1;
+  if (KIND != kGradW && BM == 256 && BN == 256 && m_tiles * n_tiles > ctx->num_cu) {  // room for the quarters of half a round
+    g.split = ctx->num_cu;
+    blocks += 3 * (cdiv(ctx->num_cu / 2, kXcds) * kXcds) + 2 * kXcds;
+  }
   SAMD_TRY(check_blocks(ctx, who, blocks));
   g.m_tiles = (int)m_tiles;
   g.n_tiles = (int)n_tiles;
@@ -307,7 +312,9 @@ int experts_panels(futhark_context *ctx, const char *who, hipStream_t stream, T 
   double least = 0;
   for (int i = 0; i < 5; i++) {
     const int64_t count = used * cdiv(mean, tiles[i].bm) * cdiv(g.N, tiles[i].bn);
-    const double t = (double)cdiv(count, 256 * tiles[i].per_cu) * tiles[i].per_cu * tiles[i].bm * tiles[i].bn / tiles[i].rate;
+    double rounds = (double)cdiv(count, 256 * tiles[i].per_cu);
+    if (i == 4 && count > 256 && count % 256 > 0 && count % 256 <= 128) rounds -= 0.5;  // a last round that is cut into quarters
+    const double t = rounds * tiles[i].per_cu * tiles[i].bm * tiles[i].bn / tiles[i].rate;
     if (i == 0 || t < least) {
       best = i;
       least = t;

@@ -54,6 +54,7 @@ struct ProductShape {
   int64_t blockB;      // elements from one block of W to the next (kForward, kGradX)
   int64_t blockC;      // elements from one block of dW to the next (kGradW)
   int X;
+  int split;           // CUs the last round of tiles is spread over, or 1: it is left as it is
   bool stream;         // the result is written past the caches
   int m_tiles, n_tiles;  // kForward / kGradX: m_tiles = upper bound over all experts; kGradW: of one block
 };
@@ -187,15 +188,18 @@ constexpr int kXcds = 8;  // workgroup i runs on die i % 8, each with an L2 of i
 // Tile `id` of m x n: every die has a run of neighbouring tiles, taken down columns of kDown tiles, so that the 32 tiles a
 // die works on at a time share 8 tiles of one operand and 4 of the other out of its L2.
 constexpr int kDown = 8;
-__device__ __forceinline__ bool place_tile(int id, int m_tiles, int n_tiles, int *m, int *n) {
-  const int tiles = m_tiles * n_tiles, per = (tiles + kXcds - 1) / kXcds;
-  const int t = (id % kXcds) * per + id / kXcds;
-  if (id / kXcds >= per || t >= tiles) return false;
+__device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles, int *m, int *n) {
   const int group = t / (kDown * n_tiles), in = t - group * (kDown * n_tiles);
   const int high = min(kDown, m_tiles - group * kDown);
   *n = in / high;
   *m = group * kDown + in - *n * high;
-  return true;
+}
+
+// The place of workgroup `id` among `tiles`: every die has a run of them.  Negative: it has none.
+__device__ __forceinline__ int place_of(int id, int tiles) {
+  const int per = (tiles + kXcds - 1) / kXcds;
+  const int t = id % kXcds * per + id / kXcds;
+  return id / kXcds < per && t < tiles ? t : -1;
 }
 
 // How many m-tiles the experts have in all.
@@ -264,38 +268,69 @@ __device__ __forceinline__ void arrived() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// Where a workgroup's tile is, and its operands.
-template <int KIND, int BM, int BN, class T, class TO, class TA, class TB>
-__device__ __forceinline__ bool place_product(TA &ta, TB &tb, TO *&out, int64_t &m0, int64_t &n0, int64_t &m_end, int64_t &summed,
-                                              TO *C, const T *A, const T *B, const int32_t *offsets, const ProductShape &g, bool skip_empty) {
-  const int id = (int)blockIdx.x;
-  int e, m, n;
+// A tile's operands: rows m0 .. and columns n0 .. of expert e's result, which ends with row m_end.
+template <int KIND, class T, class TO, class TA, class TB>
+__device__ __forceinline__ int64_t operands(TA &ta, TB &tb, TO *&out, int e, int64_t m0, int64_t n0, int64_t m_end, TO *C, const T *A, const T *B,
+                                            const int32_t *offsets, const ProductShape &g) {
   if (KIND == kGradW) {
-    // block after block of dW, each dealt to all dies: the blocks' costs differ with their experts' rows
-    const int per = (g.m_tiles * g.n_tiles + kXcds - 1) / kXcds * kXcds;
-    e = id / per;
-    if (!place_tile(id - e * per, g.m_tiles, g.n_tiles, &m, &n)) return false;
-    m0 = (int64_t)m * BM;
-    n0 = (int64_t)n * BN;
-    m_end = g.M;
-    const int64_t ra = clamped(offsets, e, g.rows), rb = clamped(offsets, e + 1, g.rows);
-    summed = same(rb > ra ? rb - ra : 0);
-    if (skip_empty && summed == 0) return false;
+    const int64_t ra = clamped(offsets, e, g.rows), rb = clamped(offsets, e + 1, g.rows), summed = same(rb > ra ? rb - ra : 0);
     ta.init(A + ra * g.ldA + m0, g.ldA, summed ? (summed - 1) * g.ldA + g.M - m0 : 0, summed, g.M - m0);
     tb.init(B + ra * g.ldB + n0, g.ldB, summed ? (summed - 1) * g.ldB + g.N - n0 : 0, summed, g.N - n0);
     out = C + (int64_t)e * g.blockC;
+    return summed;
+  }
+  ta.init(A + m0 * g.ldA, g.ldA, (m_end - m0 - 1) * g.ldA + g.K, g.K, m_end - m0);
+  const T *w = B + (int64_t)e * g.blockB;
+  if (KIND == kForward)
+    tb.init(w + n0 * g.ldB, g.ldB, (g.N - n0 - 1) * g.ldB + g.K, g.K, g.N - n0);
+  else
+    tb.init(w + n0, g.ldB, (g.K - 1) * g.ldB + g.N - n0, g.K, g.N - n0);
+  out = C;
+  return g.K;
+}
+
+// Where the workgroup's tile is.  False: it has none.
+//
+// A last round of a few tiles of 256 x 256 would leave most CUs idle for as long as any other: if it fills half of them or
+// fewer (g.split: the launch has workgroups enough) each of its tiles is cut into four of 128 x 128; *quarter = which, or -1.
+template <int KIND, int BM, int BN>
+__device__ __forceinline__ bool place_product(int *e, int64_t *m0, int64_t *n0, int64_t *m_end, int *quarter, const int32_t *offsets,
+                                              const ProductShape &g) {
+  const int id = (int)blockIdx.x;
+  int m, n;
+  *quarter = -1;
+  if (KIND == kGradW) {
+    // block after block of dW, each dealt to all dies: the blocks' costs differ with their experts' rows
+    const int per = (g.m_tiles * g.n_tiles + kXcds - 1) / kXcds * kXcds;
+    *e = id / per;
+    const int t = place_of(id - *e * per, g.m_tiles * g.n_tiles);
+    if (t < 0) return false;
+    tile_at(t, g.m_tiles, g.n_tiles, &m, &n);
+    *m0 = (int64_t)m * BM;
+    *n0 = (int64_t)n * BN;
+    *m_end = g.M;
+    return true;
+  }
+  const int m_tiles = count_tiles(offsets, g.X, g.rows, BM), tiles = m_tiles * g.n_tiles;
+  const int rest = tiles % g.split, whole = g.split > 1 && 2 * rest <= g.split ? tiles - rest : tiles;
+  const int own = (whole + kXcds - 1) / kXcds * kXcds;  // workgroups of the whole tiles
+  int t;
+  if (id < own) {
+    t = place_of(id, whole);
+    if (t < 0) return false;
   } else {
-    if (!place_tile(id, count_tiles(offsets, g.X, g.rows, BM), g.n_tiles, &m, &n)) return false;
-    if (!find_tile(offsets, g.X, g.rows, BM, m, &e, &m0, &m_end)) return false;
-    n0 = (int64_t)n * BN;
-    summed = g.K;
-    ta.init(A + m0 * g.ldA, g.ldA, (m_end - m0 - 1) * g.ldA + g.K, summed, m_end - m0);
-    const T *w = B + (int64_t)e * g.blockB;
-    if (KIND == kForward)
-      tb.init(w + n0 * g.ldB, g.ldB, (g.N - n0 - 1) * g.ldB + g.K, summed, g.N - n0);
-    else
-      tb.init(w + n0, g.ldB, (g.K - 1) * g.ldB + g.N - n0, summed, g.N - n0);
-    out = C;
+    const int q = id - own;  // the quarters of a tile go to one die
+    t = whole + q / (4 * kXcds) * kXcds + q % kXcds;
+    *quarter = q / kXcds % 4;
+    if (t >= tiles) return false;
+  }
+  tile_at(t, m_tiles, g.n_tiles, &m, &n);
+  if (!find_tile(offsets, g.X, g.rows, BM, m, e, m0, m_end)) return false;
+  *n0 = (int64_t)n * BN;
+  if (*quarter >= 0) {
+    *m0 += (*quarter >> 1) * (BM / 2);
+    *n0 += (*quarter & 1) * (BN / 2);
+    return *m0 < *m_end && *n0 < g.N;
   }
   return true;
 }
@@ -367,8 +402,11 @@ __global__ __launch_bounds__(WM *WN *kWave) void experts_any_kernel(TO *__restri
   TA ta;
   TB tb;
   TO *out;
-  int64_t m0, n0, m_end, summed;
-  if (!place_product<KIND, BM, BN>(ta, tb, out, m0, n0, m_end, summed, C, A, B, offsets, g, ADD)) return;
+  int e, quarter;
+  int64_t m0, n0, m_end;
+  if (!place_product<KIND, BM, BN>(&e, &m0, &n0, &m_end, &quarter, offsets, g)) return;
+  const int64_t summed = operands<KIND>(ta, tb, out, e, m0, n0, m_end, C, A, B, offsets, g);
+  if (ADD && summed == 0) return;
   const int wm = wave_id() / WN, wn = wave_id() % WN;
   Acc acc[NI][MI] = {};
   if (summed > 0) {
@@ -423,9 +461,14 @@ __global__ __launch_bounds__(WM *WN *kWave) void experts_any_kernel(TO *__restri
 // A stage is then read half a step later by the second four, still before the barrier behind which it is overwritten.
 //
 // ONCE: B is read past the caches, for weights that no cache could hold anyway.
+template <class T>
+struct Stages {  // an array for each stage and operand: what is read from one does not wait for loads into another
+  T *a0, *a1, *a2, *a3, *b0, *b1, *b2, *b3;
+};
+
 template <class T, class TO, int KIND, int BM, int BN, int DEPTH, int WM, int WN, bool ADD, bool ONCE>
-__global__ __launch_bounds__(WM *WN *kWave) void experts_kernel(TO *__restrict__ C, const T *__restrict__ A, const T *__restrict__ B,
-                                                                const int32_t *__restrict__ offsets, ProductShape g) {
+__device__ __forceinline__ void multiply(const Stages<T> lds, int e, int64_t m0, int64_t n0, int64_t m_end, TO *C, const T *A, const T *B,
+                                         const int32_t *offsets, const ProductShape &g) {
   constexpr int NT = WM * WN * kWave, S = 4, KK = DEPTH / 32;
   constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
   constexpr bool kPairs = WM * WN == 8;
@@ -434,14 +477,13 @@ __global__ __launch_bounds__(WM *WN *kWave) void experts_kernel(TO *__restrict__
   using Acc = typename Mfma<T>::Acc;
   using Frag = typename Mfma<T>::Frag;
   constexpr int L = TA::kLoads + TB::kLoads;
-  // an array for each stage: what is read from one does not wait for loads into another
-  __shared__ __align__(128) T a0[BM * DEPTH], a1[BM * DEPTH], a2[BM * DEPTH], a3[BM * DEPTH];
-  __shared__ __align__(128) T b0[BN * DEPTH], b1[BN * DEPTH], b2[BN * DEPTH], b3[BN * DEPTH];
+  T *const a0 = lds.a0, *const a1 = lds.a1, *const a2 = lds.a2, *const a3 = lds.a3;
+  T *const b0 = lds.b0, *const b1 = lds.b1, *const b2 = lds.b2, *const b3 = lds.b3;
   TA ta;
   TB tb;
   TO *out;
-  int64_t m0, n0, m_end, summed;
-  if (!place_product<KIND, BM, BN>(ta, tb, out, m0, n0, m_end, summed, C, A, B, offsets, g, ADD)) return;
+  const int64_t summed = operands<KIND>(ta, tb, out, e, m0, n0, m_end, C, A, B, offsets, g);
+  if (ADD && summed == 0) return;
   const int wm = wave_id() / WN, wn = wave_id() % WN;
   Acc acc[NI][MI] = {};
   // the products of stage t, which is in sa, sb; na, nb take the stage three on
@@ -512,6 +554,24 @@ __global__ __launch_bounds__(WM *WN *kWave) void experts_kernel(TO *__restrict__
   } else {
     store_product<T, TO, ADD, BM, BN, WM, WN>(out, acc, m0, n0, m_end, g);
   }
+}
+
+template <class T, class TO, int KIND, int BM, int BN, int DEPTH, int WM, int WN, bool ADD, bool ONCE>
+__global__ __launch_bounds__(WM *WN *kWave) void experts_kernel(TO *__restrict__ C, const T *__restrict__ A, const T *__restrict__ B,
+                                                                const int32_t *__restrict__ offsets, ProductShape g) {
+  __shared__ __align__(128) T a0[BM * DEPTH], a1[BM * DEPTH], a2[BM * DEPTH], a3[BM * DEPTH];
+  __shared__ __align__(128) T b0[BN * DEPTH], b1[BN * DEPTH], b2[BN * DEPTH], b3[BN * DEPTH];
+  const Stages<T> lds = {a0, a1, a2, a3, b0, b1, b2, b3};
+  int e, quarter;
+  int64_t m0, n0, m_end;
+  if (!place_product<KIND, BM, BN>(&e, &m0, &n0, &m_end, &quarter, offsets, g)) return;
+  if constexpr (KIND != kGradW && BM == 256 && BN == 256) {
+    if (quarter >= 0) {
+      multiply<T, TO, KIND, BM / 2, BN / 2, DEPTH, WM, WN, ADD, ONCE>(lds, e, m0, n0, m_end, C, A, B, offsets, g);
+      return;
+    }
+  }
+  multiply<T, TO, KIND, BM, BN, DEPTH, WM, WN, ADD, ONCE>(lds, e, m0, n0, m_end, C, A, B, offsets, g);
 }
 
 }  // namespace tok

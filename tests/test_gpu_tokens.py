@@ -289,6 +289,7 @@ def test_a_token_without_a_place_has_zeros(tk):
 EXPERTS = [([1], 0, 8, 8), ([3], 0, 1, 1), ([0, 0, 5, 0], 2, 64, 64), ([1, 2, 3, 0, 40], 3, 72, 136), ([31, 0, 33, 64, 1], 0, 200, 328),
            ([16, 17, 15] * 5, 1, 128, 256), ([100, 0, 129, 128], 7, 264, 136), ([40, 300, 1, 60], 0, 65, 77), ([5, 2, 9], 1, 1001, 13),
            ([300, 700, 1, 511], 30, 136, 520), ([2000], 0, 512, 264), ([257, 0, 1024], 5, 192, 257), ([900, 300], 9, 515, 384),
+           ([700, 500], 0, 64, 15350), ([513, 0, 511], 3, 15360, 72), ([300, 260, 10, 90], 0, 8200, 8192), ([64] * 40, 0, 96, 264),
            ([1] * 200, 0, 64, 128), ([0, 0], 10, 64, 64), ([600], 600, 96, 80)]
 
 
