@@ -165,7 +165,7 @@ struct GradPlan {
     g.chunks = cdiv(n, g.chunk);
     small = n <= kOneGroupIds && V <= ((int64_t)1 << 22);  // one workgroup clears the rows' bytes too
     const int key_bits = bits_for(V + 1) > 0 ? bits_for(V + 1) : 1;
-    const int most = small ? kSmallBits : 10;
+    const int most = small ? kSmallBits : kIdBits;
     passes = (key_bits + most - 1) / most;
     bits = (key_bits + passes - 1) / passes;
     Carve c(work);
@@ -269,7 +269,8 @@ bool direct_to_lds(const T *p, int64_t ld) {
   return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && ld <= ((int64_t)1 << 20);
 }
 
-template <class T, class TO, int KIND, int BM, int BN, int DEPTH, int WM, int WN, bool ADD, bool ONCE = false>
+// ANY: the kernel for any strides and alignment.
+template <class T, class TO, int KIND, int BM, int BN, int DEPTH, int WM, int WN, bool ADD, bool ONCE = false, bool ANY = false>
 int launch_experts(futhark_context *ctx, const char *who, hipStream_t stream, TO *C, const T *A, const T *B, const int32_t *offsets,
                    ProductShape g) {
   const int64_t n_tiles = cdiv(g.N, BN);
@@ -291,8 +292,8 @@ int launch_experts(futhark_context *ctx, const char *who, hipStream_t stream, TO
   SAMD_TRY(check_blocks(ctx, who, blocks));
   g.m_tiles = (int)m_tiles;
   g.n_tiles = (int)n_tiles;
-  if constexpr (DEPTH == 0)
-    TOK_LAUNCH(ctx, (experts_any_kernel<T, TO, KIND, BM, BN, WM, WN, ADD>), blocks, WM * WN * kWave, stream, C, A, B, offsets, g);
+  if constexpr (ANY)
+    TOK_LAUNCH(ctx, (experts_any_kernel<T, TO, KIND, BM, BN, DEPTH, WM, WN, ADD>), blocks, WM * WN * kWave, stream, C, A, B, offsets, g);
   else
     TOK_LAUNCH(ctx, (experts_kernel<T, TO, KIND, BM, BN, DEPTH, WM, WN, ADD, ONCE>), blocks, WM * WN * kWave, stream, C, A, B, offsets, g);
   return 0;
@@ -302,7 +303,10 @@ template <class T, int KIND>
 int experts_panels(futhark_context *ctx, const char *who, hipStream_t stream, T *C, const T *A, const T *B, const int32_t *offsets,
                    const ProductShape &g) {
   const bool fast = direct_to_lds(A, g.ldA) && g.K % 8 == 0 && direct_to_lds(B, g.ldB) && g.blockB % 8 == 0;
-  if (!fast) return launch_experts<T, T, KIND, 128, 128, 0, 2, 2, false>(ctx, who, stream, C, A, B, offsets, g);
+  if (!fast) {
+    if (g.rows <= 48 * g.X) return launch_experts<T, T, KIND, 32, 64, 128, 1, 4, false, false, true>(ctx, who, stream, C, A, B, offsets, g);
+    return launch_experts<T, T, KIND, 128, 128, 64, 2, 2, false, false, true>(ctx, who, stream, C, A, B, offsets, g);
+  }
   // The tile whose launch is estimated to end first: whole rounds of the card's 256 CUs, by the rate each tile reaches with
   // the card full (TFLOP/s, measured on 32 experts of 4096 x 2048).  Small tiles waste fewer rows of a small expert, large
   // ones read each operand less often: 64 rows an expert, forward: 64 x 256 136 us, 256 x 256 146; 256 rows: 244 and 180.
@@ -339,10 +343,13 @@ int experts_panels(futhark_context *ctx, const char *who, hipStream_t stream, T 
 template <class T, class TO, bool ADD>
 int experts_weights(futhark_context *ctx, const char *who, hipStream_t stream, TO *C, const T *A, const T *B, const int32_t *offsets,
                     const ProductShape &g) {
-  if (!(direct_to_lds(A, g.ldA) && direct_to_lds(B, g.ldB)))
-    return launch_experts<T, TO, kGradW, 128, 128, 0, 2, 2, ADD>(ctx, who, stream, C, A, B, offsets, g);
-  // as above: tiles enough for every CU to have a large one
-  if (g.X * cdiv(g.M, 256) * cdiv(g.N, 256) >= 256) return launch_experts<T, TO, kGradW, 256, 256, 32, 2, 4, ADD>(ctx, who, stream, C, A, B, offsets, g);
+  if (!(direct_to_lds(A, g.ldA) && direct_to_lds(B, g.ldB))) {
+    if (g.rows <= 48 * g.X) return launch_experts<T, TO, kGradW, 64, 64, 32, 2, 2, ADD, false, true>(ctx, who, stream, C, A, B, offsets, g);
+    return launch_experts<T, TO, kGradW, 128, 128, 64, 2, 2, ADD, false, true>(ctx, who, stream, C, A, B, offsets, g);
+  }
+  // as above: tiles enough for every CU to have a large one, and work in them: with few rows a tile is all writing, and two
+  // small ones on a CU overlap it better (16 rows an expert: 145 us against 150)
+  if (g.X * cdiv(g.M, 256) * cdiv(g.N, 256) >= 256 && g.rows > 64 * g.X) return launch_experts<T, TO, kGradW, 256, 256, 32, 2, 4, ADD>(ctx, who, stream, C, A, B, offsets, g);
   return launch_experts<T, TO, kGradW, 128, 128, 32, 2, 2, ADD>(ctx, who, stream, C, A, B, offsets, g);
 }
 

@@ -66,7 +66,7 @@ __device__ __forceinline__ int64_t same(int64_t v) {
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 
-// One operand's tile: R rows of the result's index, DEPTH (32 or 64) of the summed index.
+// One operand's tile: R rows of the result's index, DEPTH (32, 64 or 128) of the summed index.
 // p: element (0, 0) of the tile's first step; `rest`: elements from p to behind the operand's last one.
 template <class T, int R, int DEPTH, bool STANDING, int NT, bool FAST>
 struct Tile {
@@ -78,7 +78,7 @@ struct Tile {
   int64_t width;        // how much of the result's index there is from the tile's first on
   uint32_t off[FAST ? kLoads : 1];
   __amdgpu_buffer_rsrc_t bounds;
-  Piece<T> held[FAST ? 1 : kLoads];
+  Piece<T> held[2][FAST ? 1 : kLoads];  // not FAST: two steps on their way to LDS
 
   // the chunk that thread t's load i puts at LDS bytes (i * NT + t) * 16: its row in memory and its first column there
   static __device__ __forceinline__ void source(int i, int t, int *row, int *col) {
@@ -97,7 +97,7 @@ struct Tile {
   }
   // ds_read_b128 serves 16 lanes at a time, over 64 banks: lanes 0-3, 12-15 and 20-27, then 4-11, 16-19 and 28-31, and the
   // same of the upper half.  Either set has to find its rows' chunks in 16 different places.
-  static __device__ __forceinline__ int twist(int r) { return DEPTH == 64 ? (r >> 1) & 7 : (4 - (r >> 2)) & 3; }
+  static __device__ __forceinline__ int twist(int r) { return DEPTH == 128 ? r & 15 : DEPTH == 64 ? (r >> 1) & 7 : (4 - (r >> 2)) & 3; }
   static __device__ __forceinline__ int spread(int k) { return (k & 3) | (((k >> 3) & 1) << 2); }
 
   __device__ __forceinline__ void init(const T *base, int64_t ld_, int64_t rest_, int64_t summed_, int64_t width_) {
@@ -142,6 +142,7 @@ struct Tile {
   }
 
   // Not FAST: the step at summed index k0 into registers, and from there into lds.
+  template <int SET>
   __device__ __forceinline__ void bring(int64_t k0) {
     const int64_t step = STANDING ? k0 * ld : k0;
 #pragma unroll
@@ -149,12 +150,13 @@ struct Tile {
       int r, c;
       source(i, threadIdx.x, &r, &c);
       const int64_t left = STANDING ? (k0 + r < summed ? width - c : 0) : (r < width ? summed - k0 - c : 0);
-      held[FAST ? 0 : i] = load_piece(p + step + r * ld + c, left);
+      held[SET][FAST ? 0 : i] = load_piece(p + step + r * ld + c, left);
     }
   }
+  template <int SET>
   __device__ __forceinline__ void put(T *lds) {
 #pragma unroll
-    for (int i = 0; i < kLoads; i++) __builtin_memcpy((char *)lds + (i * NT + (int)threadIdx.x) * 16, &held[FAST ? 0 : i], 16);
+    for (int i = 0; i < kLoads; i++) __builtin_memcpy((char *)lds + (i * NT + (int)threadIdx.x) * 16, &held[SET][FAST ? 0 : i], 16);
   }
 
   // Fragment of rows r0 .. r0+15 and summed index 32 kk .. 32 kk + 31: lane l has row r0 + l % 16, eight k from 8 (l / 16) on.
@@ -352,8 +354,8 @@ __device__ __forceinline__ void store_product(TO *out, const Acc (&acc)[NI][MI],
 }
 
 // Rounded to 16 bits: through `mine`, LDS that only this wave uses, so that a row leaves the wave in pieces of 16 bytes that
-// lie side by side (a wave's 64 columns are a cache line; written four columns a lane, blocks of 4096 x 2048 for few rows took
-// 214 us where this takes 100).  The pieces of a row are permuted by the row's number: the lanes that write the same
+// lie side by side (a wave's 64 columns are a cache line; written four columns a lane, 32 blocks of 4096 x 2048 for few rows took
+// 214 us where this takes 150).  The pieces of a row are permuted by the row's number: the lanes that write the same
 // columns of 16 rows would all meet in a few banks.
 template <class T, int BM, int BN, int WM, int WN, class Acc, int NI, int MI>
 __device__ __forceinline__ void store_rounded(T *mine, T *out, const Acc (&acc)[NI][MI], int64_t m0, int64_t n0, int64_t m_end, const ProductShape &g) {
@@ -385,13 +387,14 @@ __device__ __forceinline__ void store_rounded(T *mine, T *out, const Acc (&acc)[
   }
 }
 
-// Any strides and alignment: the next step's chunks wait in registers while this one's products run.
+// Any strides and alignment: a step's chunks are loaded into registers two steps before its products, and put into one of
+// two LDS buffers one step before.
 // A wave computes BM/WM x BN/WN of the tile, B's fragment as the first operand: a lane then holds four neighbouring
 // columns of one row of the result.
-template <class T, class TO, int KIND, int BM, int BN, int WM, int WN, bool ADD>
+template <class T, class TO, int KIND, int BM, int BN, int DEPTH, int WM, int WN, bool ADD>
 __global__ __launch_bounds__(WM *WN *kWave) void experts_any_kernel(TO *__restrict__ C, const T *__restrict__ A, const T *__restrict__ B,
                                                                     const int32_t *__restrict__ offsets, ProductShape g) {
-  constexpr int NT = WM * WN * kWave, DEPTH = 64;
+  constexpr int NT = WM * WN * kWave;
   constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
   using TA = Tile<T, BM, DEPTH, KIND == kGradW, NT, false>;
   using TB = Tile<T, BN, DEPTH, KIND != kForward, NT, false>;
@@ -409,35 +412,39 @@ __global__ __launch_bounds__(WM *WN *kWave) void experts_any_kernel(TO *__restri
   if (ADD && summed == 0) return;
   const int wm = wave_id() / WN, wn = wave_id() % WN;
   Acc acc[NI][MI] = {};
-  if (summed > 0) {
-    ta.bring(0);
-    tb.bring(0);
-    ta.put(sa[0]);
-    tb.put(sb[0]);
-  }
-  int at = 0;
-  for (int64_t k0 = 0; k0 < summed; k0 += DEPTH, at ^= 1) {
+  // the products of the step in buffer SET; the next step goes from registers into the other one
+  const auto step = [&](auto set, int64_t k0) {
+    constexpr int SET = decltype(set)::value;
     __syncthreads();  // this step's slices are there, and nobody reads the other buffer any more
-    const bool more = k0 + DEPTH < summed;
-    if (more) {
-      ta.bring(k0 + DEPTH);
-      tb.bring(k0 + DEPTH);
-    }
+    ta.template put<SET ^ 1>(sa[SET ^ 1]);
+    tb.template put<SET ^ 1>(sb[SET ^ 1]);
+    ta.template bring<SET ^ 1>(k0 + 3 * DEPTH);  // nothing is read behind the end
+    tb.template bring<SET ^ 1>(k0 + 3 * DEPTH);
 #pragma unroll
     for (int kk = 0; kk < DEPTH / 32; kk++) {
       Frag fa[MI], fb[NI];
 #pragma unroll
-      for (int i = 0; i < MI; i++) fa[i] = TA::fragment(sa[at], wm * (BM / WM) + i * 16, kk);
+      for (int i = 0; i < MI; i++) fa[i] = TA::fragment(sa[SET], wm * (BM / WM) + i * 16, kk);
 #pragma unroll
-      for (int j = 0; j < NI; j++) fb[j] = TB::fragment(sb[at], wn * (BN / WN) + j * 16, kk);
+      for (int j = 0; j < NI; j++) fb[j] = TB::fragment(sb[SET], wn * (BN / WN) + j * 16, kk);
 #pragma unroll
       for (int j = 0; j < NI; j++)
 #pragma unroll
         for (int i = 0; i < MI; i++) acc[j][i] = Mfma<T>::go(fb[j], fa[i], acc[j][i]);
     }
-    if (more) {
-      ta.put(sa[at ^ 1]);
-      tb.put(sb[at ^ 1]);
+  };
+  if (summed > 0) {
+    ta.template bring<0>(0);
+    tb.template bring<0>(0);
+    ta.template bring<1>(DEPTH);
+    tb.template bring<1>(DEPTH);
+    ta.template put<0>(sa[0]);
+    tb.template put<0>(sb[0]);
+    ta.template bring<0>(2 * DEPTH);
+    tb.template bring<0>(2 * DEPTH);
+    for (int64_t k0 = 0; k0 < summed; k0 += 2 * DEPTH) {  // a step behind the last multiplies zeros
+      step(std::integral_constant<int, 0>(), k0);
+      step(std::integral_constant<int, 1>(), k0 + DEPTH);
     }
   }
   if constexpr (std::is_same<T, TO>::value && !ADD) {

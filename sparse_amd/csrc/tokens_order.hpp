@@ -18,6 +18,7 @@ namespace tok {
 
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxBins = kMaxExperts + 1;  // the last bin: choices that name no expert
+constexpr int kIdBits = 10, kIdBins = 1 << kIdBits;  // of a split pass over ids, at most
 constexpr int kOneGroupChoices = 4096, kOneGroupIds = 2048;  // what one workgroup orders by itself
 constexpr int kSplitWaves = 8, kSplitThreads = kSplitWaves * kWave;
 constexpr int kTile = kSplitThreads;       // items a workgroup of a split pass places at a time
@@ -150,7 +151,7 @@ struct Digits {
 template <int BY, class I>
 __global__ __launch_bounds__(kSplitThreads) void digit_count_kernel(Digits<BY, I> d, int64_t per_group, int bins, int *__restrict__ hist,
                                                                     uint32_t *__restrict__ clear, int64_t clear_words) {
-  __shared__ int cnt[kMaxBins];
+  __shared__ int cnt[BY == 0 ? kMaxBins : kIdBins];
   for (int64_t k = (int64_t)blockIdx.x * kSplitThreads + threadIdx.x; k < clear_words; k += (int64_t)gridDim.x * kSplitThreads) clear[k] = 0;
   for (int b = threadIdx.x; b < bins; b += kSplitThreads) cnt[b] = 0;
   __syncthreads();
@@ -173,8 +174,9 @@ template <int BY, class I>
 __global__ __launch_bounds__(kSplitThreads) void digit_place_kernel(Digits<BY, I> d, int64_t per_group, int bins, int bits,
                                                                     const int *__restrict__ hist, PassOut o) {
   constexpr int IPL = kTile / kSplitThreads;
-  __shared__ int cnt[kSplitWaves * kMaxBins];
-  __shared__ int base[kMaxBins];
+  constexpr int kBins = BY == 0 ? kMaxBins : kIdBins;
+  __shared__ int cnt[kSplitWaves * kBins];
+  __shared__ int base[kBins];
   __shared__ int wave_total[kSplitWaves];
   const int groups = (int)gridDim.x, g = (int)blockIdx.x;
   const int64_t i0 = (int64_t)g * per_group, i1 = i0 + per_group < d.n ? i0 + per_group : d.n;
