@@ -609,8 +609,8 @@ int sparse_amd_dcsr_f64_smvm(struct sparse_amd_group *g, struct sparse_amd_dvec_
  *     that an expert's places lie side by side, in the order of the batch; dispatch and combine are the products with that
  *     permutation and with its weighted transpose, experts the product with the block-diagonal matrix of the experts' blocks.
  * Conventions of this group, where they differ from the rest of this header:
- *   - arguments are plain device pointers; a panel of rows has a row stride (`ld...`, in elements) of at least its width and
- *     no alignment beyond its elements';
+ *   - arguments are plain device pointers; a panel of rows has a row stride (`ld...`, in elements) and no alignment beyond its
+ *     elements'.  The rows of a result lie apart (ld >= width); rows that are only read may have any stride, zero included;
  *   - every call names the HIP stream it runs on (NULL: the null stream) and touches neither the context's stream nor its
  *     memory: it allocates nothing, never waits, keeps nothing between calls, and may be captured into a graph.  What needs
  *     a workspace takes it as an argument (256-byte aligned, at least ..._workspace bytes, free for other use when the
@@ -620,7 +620,7 @@ int sparse_amd_dcsr_f64_smvm(struct sparse_amd_group *g, struct sparse_amd_dvec_
  *   - indices that come in have `id_bits` = 32 or 64 bits.  An id outside 0 .. V-1, or an expert outside 0 .. X-1, selects
  *     nothing: a row of zeros, no place (pos = -1), no gradient;
  *   - results are the same bits on every call with the same arguments;
- *   - a result may not overlap another result or an argument.
+ *   - a result may not overlap another result or an argument, nor lie between its rows.
  * Errors: as everywhere in this header (non-zero, text in futhark_context_get_error); nothing is launched then. */
 #define SPARSE_AMD_F32 0
 #define SPARSE_AMD_F16 1
@@ -633,7 +633,8 @@ int sparse_amd_tokens_lookup(struct futhark_context *ctx, void *stream, int type
 int sparse_amd_tokens_lookup_dots(struct futhark_context *ctx, void *stream, int type, float *dvals, const void *dy,
                                   int64_t ldy, const void *table, int64_t V, int64_t D, int64_t ldt, const void *ids,
                                   int id_bits, int64_t n, float scale);
-/* dtable[v] = sum over i with ids[i] = v of scale vals[i] dy[i], added in the order of i: lookup's gradient by the table.
+/* dtable[v] = sum over i with ids[i] = v of scale vals[i] dy[i], added in an order that the ids alone decide: lookup's gradient
+ * by the table.
  * accumulate = 0: every row of dtable is written (zeros where no id names it); else the sums are added to dtable, and rows
  * no id names are not touched.  out_type: type or SPARSE_AMD_F32.  V and n are at most 2^31 - 2. */
 int sparse_amd_tokens_lookup_grad(struct futhark_context *ctx, void *stream, int type, int out_type, int accumulate,

@@ -35,6 +35,7 @@ int need_device(futhark_context *ctx) {
 // Runs `body` with the context locked and its device current; no exception leaves.
 template <class F>
 int entry(futhark_context *ctx, F body) {
+  if (!ctx) return 1;
   try {
     OnDevice on(ctx);
     return body();
@@ -83,12 +84,14 @@ struct Panel {
   int64_t bytes() const { return rows > 0 && cols > 0 ? ((rows - 1) * ld + cols) * size : 0; }
 };
 
-// Every panel has a place and a stride that keeps its rows apart; the results (the first `outs` panels) share no byte
-// with each other or with what is read.
+// Every panel has a place; the results (the first `outs` panels) have strides that keep their rows apart and share no byte
+// with each other or with what is read.  Rows that are only read may lie over each other (a stride of zero: one row for all).
 int check_panels(futhark_context *ctx, const char *who, int outs, std::initializer_list<Panel> panels) {
+  int k = 0;
   for (const Panel &a : panels) {
     if (a.rows < 0 || a.cols < 0) return set_error(ctx, "%s: %s has a negative size", who, a.name);
-    if (a.rows > 1 && a.ld < a.cols) return set_error(ctx, "%s: the rows of %s are %lld apart and %lld long", who, a.name, (long long)a.ld, (long long)a.cols);
+    if (a.rows > 1 && a.ld < 0) return set_error(ctx, "%s: %s has a negative stride", who, a.name);
+    if (k++ < outs && a.rows > 1 && a.ld < a.cols) return set_error(ctx, "%s: the rows of %s are %lld apart and %lld long", who, a.name, (long long)a.ld, (long long)a.cols);
     if (a.ld > ((int64_t)1 << 40) || a.rows > ((int64_t)1 << 40) || a.cols > ((int64_t)1 << 40) ||
         (a.rows > 0 && a.ld > 0 && a.rows > ((int64_t)1 << 56) / a.ld))
       return set_error(ctx, "%s: %s is too large", who, a.name);
@@ -264,9 +267,10 @@ int sum_ids_as(futhark_context *ctx, hipStream_t stream, bool add, TO *dE, const
 }
 
 // ---------------------------------------------------------------- experts
+// Rows that begin on 16 bytes, and apart from each other: the buffer's end is what tells rows behind the last one.
 template <class T>
-bool direct_to_lds(const T *p, int64_t ld) {
-  return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && ld <= ((int64_t)1 << 20);
+bool direct_to_lds(const T *p, int64_t ld, int64_t width) {
+  return (uintptr_t)p % 16 == 0 && ld >= width && ld % 8 == 0 && ld <= ((int64_t)1 << 20);
 }
 
 // ANY: the kernel for any strides and alignment.
@@ -302,7 +306,7 @@ int launch_experts(futhark_context *ctx, const char *who, hipStream_t stream, TO
 template <class T, int KIND>
 int experts_panels(futhark_context *ctx, const char *who, hipStream_t stream, T *C, const T *A, const T *B, const int32_t *offsets,
                    const ProductShape &g) {
-  const bool fast = direct_to_lds(A, g.ldA) && g.K % 8 == 0 && direct_to_lds(B, g.ldB) && g.blockB % 8 == 0;
+  const bool fast = direct_to_lds(A, g.ldA, g.K) && g.K % 8 == 0 && direct_to_lds(B, g.ldB, KIND == kForward ? g.K : g.N) && g.blockB % 8 == 0;
   if (!fast) {
     if (g.rows <= 48 * g.X) return launch_experts<T, T, KIND, 32, 64, 128, 1, 4, false, false, true>(ctx, who, stream, C, A, B, offsets, g);
     return launch_experts<T, T, KIND, 128, 128, 64, 2, 2, false, false, true>(ctx, who, stream, C, A, B, offsets, g);
@@ -343,7 +347,7 @@ int experts_panels(futhark_context *ctx, const char *who, hipStream_t stream, T 
 template <class T, class TO, bool ADD>
 int experts_weights(futhark_context *ctx, const char *who, hipStream_t stream, TO *C, const T *A, const T *B, const int32_t *offsets,
                     const ProductShape &g) {
-  if (!(direct_to_lds(A, g.ldA) && direct_to_lds(B, g.ldB))) {
+  if (!(direct_to_lds(A, g.ldA, g.M) && direct_to_lds(B, g.ldB, g.N))) {
     if (g.rows <= 48 * g.X) return launch_experts<T, TO, kGradW, 64, 64, 32, 2, 2, ADD, false, true>(ctx, who, stream, C, A, B, offsets, g);
     return launch_experts<T, TO, kGradW, 128, 128, 64, 2, 2, ADD, false, true>(ctx, who, stream, C, A, B, offsets, g);
   }
@@ -352,6 +356,9 @@ int experts_weights(futhark_context *ctx, const char *who, hipStream_t stream, T
   if (g.X * cdiv(g.M, 256) * cdiv(g.N, 256) >= 256 && g.rows > 64 * g.X) return launch_experts<T, TO, kGradW, 256, 256, 32, 2, 4, ADD>(ctx, who, stream, C, A, B, offsets, g);
   return launch_experts<T, TO, kGradW, 128, 128, 32, 2, 2, ADD>(ctx, who, stream, C, A, B, offsets, g);
 }
+
+// Elements from a block's first to behind its last one.
+int64_t block_span(int64_t F, int64_t D, int64_t ld) { return F > 0 && D > 0 ? (F - 1) * ld + D : 0; }
 
 int check_experts(futhark_context *ctx, const char *who, int64_t rows, int64_t X, int64_t F, int64_t D, const int32_t *offsets) {
   if (rows < 0 || F < 0 || D < 0) return set_error(ctx, "%s: negative size", who);
@@ -567,9 +574,8 @@ int sparse_amd_tokens_experts(struct futhark_context *ctx, void *stream, int typ
     SAMD_TRY(check_experts(ctx, who, rows, X, F, D, offsets));
     return by_type16(ctx, who, type, [&](auto t) -> int {
       typedef typename decltype(t)::type T;
-      if (X > 1 && blockw < (F > 0 ? (F - 1) * ldw + D : 0)) return set_error(ctx, "%s: the blocks of w overlap", who);
       SAMD_TRY(check_panels(ctx, who, 1, {{"the result", ys, rows, F, ldy, 2}, {"xs", xs, rows, D, ldx, 2},
-                                          {"w", w, X, F > 0 ? (F - 1) * ldw + D : 0, X > 1 ? blockw : (F - 1) * ldw + D, 2}, {"a block of w", w, F, D, ldw, 2},
+                                          {"w", w, X, block_span(F, D, ldw), X > 1 ? blockw : block_span(F, D, ldw), 2}, {"a block of w", w, F, D, ldw, 2},
                                           {"offsets", offsets, 1, X + 1, X + 1, 4}}));
       if (rows == 0 || F == 0) return 0;
       ProductShape g = {};
@@ -588,9 +594,8 @@ int sparse_amd_tokens_experts_grad_x(struct futhark_context *ctx, void *stream, 
     SAMD_TRY(check_experts(ctx, who, rows, X, F, D, offsets));
     return by_type16(ctx, who, type, [&](auto t) -> int {
       typedef typename decltype(t)::type T;
-      if (X > 1 && blockw < (F > 0 ? (F - 1) * ldw + D : 0)) return set_error(ctx, "%s: the blocks of w overlap", who);
       SAMD_TRY(check_panels(ctx, who, 1, {{"the result", dxs, rows, D, ldx, 2}, {"dys", dys, rows, F, ldy, 2},
-                                          {"w", w, X, F > 0 ? (F - 1) * ldw + D : 0, X > 1 ? blockw : (F - 1) * ldw + D, 2}, {"a block of w", w, F, D, ldw, 2},
+                                          {"w", w, X, block_span(F, D, ldw), X > 1 ? blockw : block_span(F, D, ldw), 2}, {"a block of w", w, F, D, ldw, 2},
                                           {"offsets", offsets, 1, X + 1, X + 1, 4}}));
       if (rows == 0 || D == 0) return 0;
       ProductShape g = {};
@@ -611,10 +616,10 @@ int sparse_amd_tokens_experts_grad_w(struct futhark_context *ctx, void *stream, 
       return set_error(ctx, "%s: the gradient has the rows' element type or 32 bits", who);
     return by_type16(ctx, who, type, [&](auto t) -> int {
       typedef typename decltype(t)::type T;
-      if (X > 1 && blockw < (F > 0 ? (F - 1) * ldw + D : 0)) return set_error(ctx, "%s: the blocks of dw overlap", who);
-      SAMD_TRY(check_panels(ctx, who, 1, {{"the result", dw, X, F > 0 ? (F - 1) * ldw + D : 0, X > 1 ? blockw : (F - 1) * ldw + D, type_size(out_type)},
+      if (X > 1 && blockw < block_span(F, D, ldw)) return set_error(ctx, "%s: the blocks of dw overlap", who);
+      SAMD_TRY(check_panels(ctx, who, 1, {{"the result", dw, X, block_span(F, D, ldw), X > 1 ? blockw : block_span(F, D, ldw), type_size(out_type)},
                                           {"dys", dys, rows, F, ldy, 2}, {"xs", xs, rows, D, ldx, 2}, {"offsets", offsets, 1, X + 1, X + 1, 4}}));
-      SAMD_TRY(check_panels(ctx, who, 0, {{"a block of the result", dw, F, D, ldw, type_size(out_type)}}));
+      SAMD_TRY(check_panels(ctx, who, 1, {{"a block of the result", dw, F, D, ldw, type_size(out_type)}}));
       if (F == 0 || D == 0) return 0;
       ProductShape g = {};
       g.rows = rows; g.M = F; g.N = D; g.ldA = ldy; g.ldB = ldx; g.ldC = ldw; g.blockC = blockw; g.X = (int)X;

@@ -14,12 +14,13 @@ Neighbours of sparse_amd.mono (a record of col_idx[n] and vals[n], mono.fut:95) 
 call is one entry of include/sparse_amd.h, group (7), where the formulas stand.  What differs from the other modules:
 
 * arguments and results are torch CUDA tensors (numpy knows no bf16), on the context's device; a row of a panel is
-  contiguous, its rows may be any stride apart;
+  contiguous, its rows may be any stride apart (expanded rows too, where they are only read);
 * a call runs on torch's current stream of that device, like torch's own operations, whatever stream the context is on; it
   allocates from torch's allocator only, never waits, and may be captured into a graph.  Rows of a result it does not
   define (behind the last routed slot) are whatever the memory held, or what `out` held;
 * an id or an expert out of range selects nothing (row of zeros, place -1); there is no error for it, since that would
   have to wait for the device;
+* `out` shares no memory with an argument;
 * nothing is recorded for torch's autograd: the gradients are calls of their own.
 
 Arguments that do not fit (type, shape, device, overlap) raise SparseError before anything is launched.
@@ -149,6 +150,8 @@ class mk_tokens:
         return dtype, self._code if dtype == self._dtype else 0
 
     def _call(self, f, *args):
+        if not self.ctx.h:
+            raise SparseError("the context is closed")
         if f(self.ctx.h, _current_stream(self._dev), *args):
             raise SparseError(self.ctx.error() or "entry point failed")
 
@@ -159,6 +162,13 @@ class mk_tokens:
             return None, None
         w = torch.empty(size, dtype=torch.uint8, device=self._device)
         return w, w.data_ptr()
+
+    @staticmethod
+    def _as_rows(a, ids):
+        """ids.shape + (D,) as the panel [ids.numel(), D]."""
+        if isinstance(a, torch.Tensor) and ids.dim() != 1 and a.shape[:-1] == ids.shape and a.is_contiguous():
+            return a.view(ids.numel(), a.shape[-1])
+        return a
 
     # ---- one entry per row
     def lookup(self, E, ids, vals=None, scale=1.0, out=None):
@@ -173,13 +183,14 @@ class mk_tokens:
 
     def lookup_grad(self, dy, ids, V, vals=None, scale=1.0, out=None, accumulate=False, dtype=None):
         """lookup's gradient by the table: dE[v] = the sum of scale * vals[i] * dy[i] over the i with ids[i] = v, added in
-        32 bits in the order of the batch.  dy: [ids.numel(), D] (or ids.shape + (D,), contiguous).  accumulate: added to
+        32 bits in an order that the ids alone decide.  dy: [ids.numel(), D] (or ids.shape + (D,), contiguous).  accumulate: added to
         `out` instead of written over it; rows no id names are then not touched.  dtype (without `out`): the module's
         element type or torch.float32."""
         i, bits, n = self._ids(ids, "ids")
-        if isinstance(dy, torch.Tensor) and dy.dim() != 2 and dy.is_contiguous() and dy.dim() > 0:
-            dy = dy.view(n, dy.shape[-1])
-        g, ldg, _, D = self._panel(dy, "dy", rows=n)
+        V = int(V)
+        if V < 0:
+            raise SparseError("lookup_grad: %d rows" % V)
+        g, ldg, _, D = self._panel(self._as_rows(dy, ids), "dy", rows=n)
         f = self._flat(vals, "vals", (torch.float32,), ids.shape) if vals is not None else None
         if accumulate and out is None:
             raise SparseError("lookup_grad: accumulate needs `out`")
@@ -194,9 +205,7 @@ class mk_tokens:
         """lookup's gradient by vals: scale * <dy[i], E[ids[i]]>, float32, shape of ids."""
         i, bits, n = self._ids(ids, "ids")
         e, lde, V, D = self._panel(E, "E")
-        if isinstance(dy, torch.Tensor) and dy.dim() != 2 and dy.is_contiguous():
-            dy = dy.view(n, D) if dy.numel() == n * D else dy
-        g, ldg, _, _ = self._panel(dy, "dy", rows=n, cols=D)
+        g, ldg, _, _ = self._panel(self._as_rows(dy, ids), "dy", rows=n, cols=D)
         d = torch.empty(ids.shape, dtype=torch.float32, device=ids.device)
         self._call(self._c_lookup_dots, self._code, d.data_ptr(), g, ldg, e, V, D, lde, i, bits, n, scale)
         return d

@@ -351,6 +351,83 @@ def test_an_experts_nan_stays_with_it(tk):
     assert torch.isfinite(dW[0]).all() and torch.isfinite(dW[2]).all() and not torch.isfinite(dW[1]).any()
 
 
+@pytest.mark.parametrize("D,F", [(0, 16), (16, 0), (0, 0)])
+def test_products_of_nothing(tk, D, F):
+    r = routed(tk("bf16"), gen(1), [3, 0, 2], 1)
+    z = lambda *s: torch.zeros(s, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    assert not tk("bf16").experts(z(6, D), z(3, F, D), r, out=torch.zeros_like(z(6, F)) + 1)[:5].any()
+    assert not tk("bf16").experts_grad_x(z(6, F), z(3, F, D), r, out=z(6, D) + 1)[:5].any()
+    assert tk("bf16").experts_grad_w(z(6, F), z(6, D), r).shape == (3, F, D)
+    none = tk("bf16").route(torch.zeros(4, 0, device="cuda", dtype=torch.int64), 3)
+    assert not none.offsets.any() and not tk("bf16").combine(z(0, 16), none, torch.zeros(4, 0, device="cuda")).any()
+    assert tk("bf16").dispatch(z(4, 16), none).shape == (0, 16) and not tk("bf16").experts_grad_w(z(0, 4), z(0, 8), none).any()
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_products_keep_small_values(tk, t):
+    """Values below the type's smallest normal one are values too, in and out of the matrix cores."""
+    r = routed(tk(t), gen(2), [20, 30], 0)
+    small = 2.0 ** -20 if t == "f16" else 2.0 ** -130
+    x = torch.full((50, 64), small, device="cuda").to(DT[t])
+    assert (x == small).all()
+    W = torch.ones(2, 40, 64, device="cuda", dtype=DT[t])
+    assert (tk(t).experts(x, W, r) == 64 * small).all()
+    assert (tk(t).experts_grad_x(torch.ones(50, 40, device="cuda", dtype=DT[t]), W * x[0, 0], r) == 40 * small).all()
+
+
+def test_inputs_that_are_one_row_for_all(tk):
+    """Expanded rows and blocks: what the gradient of a sum over rows, or experts with the same weights, look like."""
+    g, k = gen(4), tk("bf16")
+    r = routed(k, g, [40, 3, 90], 2)
+    row, W = normal(g, (1, 64), DT["bf16"]), normal(g, (1, 72, 64), DT["bf16"])
+    xs, Ws = row.expand(135, 64), W.expand(3, 72, 64)
+    assert torch.equal(k.experts(xs, Ws, r)[:133], k.experts(xs.contiguous(), Ws.contiguous(), r)[:133])
+    dys = normal(g, (1, 72), DT["bf16"]).expand(135, 72)
+    assert torch.equal(k.experts_grad_x(dys, Ws, r)[:133], k.experts_grad_x(dys.contiguous(), Ws.contiguous(), r)[:133])
+    assert torch.equal(k.experts_grad_w(dys, xs, r), k.experts_grad_w(dys.contiguous(), xs.contiguous(), r))
+    ids = make_ids(g, 500, 40, "skew", 64)
+    assert torch.equal(k.lookup_grad(row.expand(500, 64), ids, 40), k.lookup_grad(row.expand(500, 64).contiguous(), ids, 40))
+    assert torch.equal(k.combine(xs, r), k.combine(xs.contiguous(), r))
+
+
+def test_far_rows(tk):
+    """Tables and blocks whose elements are counted beyond 32 bits."""
+    k, g = tk("bf16"), gen(8)
+    V, D = 4300000, 1024                                           # 4.4e9 elements
+    E = torch.empty(V, D, device="cuda", dtype=torch.bfloat16)
+    ids = torch.tensor([V - 1, 0, V - 7, 4194304, 4194303], device="cuda")
+    E[ids] = normal(g, (5, D), torch.bfloat16)
+    want = E[ids]
+    assert torch.equal(k.lookup(E, ids), want)
+    dy = normal(g, (5, D), torch.bfloat16)
+    k.lookup_grad(dy, ids, V, out=E, accumulate=True)
+    assert torch.equal(E[ids], (want.float() + dy.float()).bfloat16())
+    many = ids.repeat(100)                                         # through the ordered path
+    E[ids] = 0
+    k.lookup_grad(dy.repeat(100, 1), many, V, out=E, accumulate=True)
+    assert torch.equal(E[ids], (100.0 * dy.double()).bfloat16())
+    xs, w = E[:4200000], torch.full((4200000, 1), 2.0, device="cuda")
+    r = k.route(torch.zeros(4200000, 1, device="cuda", dtype=torch.int32), 1)
+    xs[-3:] = want[:3]
+    y = k.combine(xs, r, w)
+    assert torch.equal(y[-3:], want[:3] * 2)
+    out = k.dispatch(y, r, out=xs)
+    assert torch.equal(out[-3:], want[:3] * 2)
+    W = torch.empty(5, 16384, 65536, device="cuda", dtype=torch.bfloat16)   # 5.4e9 elements
+    W[4, -40:] = 0
+    W[4, -40:, 5] = 3.0
+    r = routed(k, g, [0, 0, 0, 0, 2], 0)
+    x = torch.zeros(2, 65536, device="cuda", dtype=torch.bfloat16)
+    x[:, 5] = 2.0
+    y = k.experts(x, W, r)
+    assert (y[:, -40:] == 6.0).all()
+    dys = torch.zeros(2, 16384, device="cuda", dtype=torch.bfloat16)
+    dys[:, -1] = 1.0
+    assert (k.experts_grad_x(dys, W.nan_to_num_(0.0, 0.0, 0.0), r)[:, 5] == 3.0).all()
+    k.experts_grad_w(dys, x, r, out=W)
+    assert (W[4, -1, 5] == 4.0) and not W[4, -2].any() and not W[0].any()
+
+
 # ------------------------------------------------------------------------------------------------ gradients against differences
 def test_gradients_are_the_differences(tk):
     """Every operator is linear in each argument: with small whole numbers nothing is rounded, and a difference over a step
@@ -422,7 +499,7 @@ def test_a_layer_of_experts_and_its_gradients(tk):
     out = (torch.matmul(blocks, x[:, None, :, None]).squeeze(-1) * torch.where(use, w, 0.0)[..., None]).sum(1)
     out.backward(s["dy"].double())
     for got, want, roundings in ((y, out, 2), (dw, w.grad, 1), (dW, W.grad, 1), (dx, x.grad, 3), (dE, E.grad, 3)):
-        off = float((got.double() - want).norm() / want.norm())
+        off = float((got.double() - want.detach()).norm() / want.detach().norm())
         assert off <= roundings * 2.0 ** -8, off
 
 
@@ -492,7 +569,9 @@ def test_refusals_on_tensors(tk):
                         ("rows|expected", lambda: k.dispatch(E, r)), ("overlaps", lambda: k.dispatch(x, r, out=E[:4])), ("shape", lambda: k.combine(ys, r, w[:1])),
                         ("no weights", lambda: k.combine_grad(x, ys, r, None)), ("blocks for", lambda: k.experts(ys, W[:2], r)), ("expected", lambda: k.experts(ys, W[:, :, :8], r)),
                         ("16-bit", lambda: tk("f32").experts(ys.float(), W.float(), r)), ("experts", lambda: k.route(ids.view(2, 2), 1025)),
-                        ("Routing", lambda: k.experts(ys, W, None)), ("overlap", lambda: k.experts_grad_w(E[:4, :8], ys, r, out=W[:1].expand(3, 8, 16)))]:
+                        ("Routing", lambda: k.experts(ys, W, None)), ("overlap", lambda: k.experts_grad_w(E[:4, :8], ys, r, out=W[:1].expand(3, 8, 16))),
+                        ("apart", lambda: k.lookup(E, ids, out=torch.zeros(1, 16, device="cuda", dtype=torch.bfloat16).expand(4, 16))), ("-1 rows", lambda: k.lookup_grad(ys, ids, -1)),
+                        ("expected", lambda: k.lookup_grad(ys.view(2, 2, 16), ids, 9))]:
         with pytest.raises(SparseError, match=words):
             call()
     assert not k.lookup(E, ids).any()                              # and the module still works

@@ -67,7 +67,7 @@ def test_what_passes_the_checks_asks_for_a_device(call, f):
 
 
 REFUSED = [
-    (lookup, dict(type=7), "element type"), (lookup, dict(bits=16), "32 or 64 bits"), (lookup, dict(ldt=63), "apart"),
+    (lookup, dict(type=7), "element type"), (lookup, dict(bits=16), "32 or 64 bits"), (lookup, dict(ldt=-1), "negative stride"),
     (lookup, dict(ldy=63), "apart"), (lookup, dict(n=-1), "negative"), (lookup, dict(y=None), "null"), (lookup, dict(ids=None), "null"),
     (lookup, dict(table=None), "null"), (lookup, dict(y=B + 64), "overlaps"), (lookup, dict(y=C), "overlaps"), (lookup, dict(y=A + 1), "aligned"),
     (lookup, dict(vals=A + 8), "overlaps"), (lookup, dict(ids=C + 4), "aligned"), (lookup, dict(ldt=1 << 50), "too large"),
@@ -76,9 +76,9 @@ REFUSED = [
     (grad, dict(n=1 << 31), "31 bits"), (grad, dict(bits=8), "32 or 64 bits"),
     (route, dict(X=0), "experts"), (route, dict(X=1025), "experts"), (route, dict(n=-1), "negative"), (route, dict(n=1 << 31), "31 bits"),
     (route, dict(pos=A), "overlaps"), (route, dict(src=B), "overlaps"), (route, dict(n=100000, size=64), "workspace of"), (route, dict(offsets=None), "null"),
-    (combine, dict(K=-1), "places a row"), (combine, dict(ldys=10), "apart"), (combine, dict(y=B), "overlaps"), (combine, dict(pos=None), "null"),
-    (experts, dict(type=F32), "16-bit"), (experts, dict(X=2000), "experts"), (experts, dict(offsets=None), "null"), (experts, dict(block=2000), "overlap"),
-    (experts, dict(ldw=60), "apart"), (experts, dict(ys=B), "overlaps"), (experts, dict(rows=-1), "negative"), (experts, dict(F=1 << 31), "too large"),
+    (combine, dict(K=-1), "places a row"), (combine, dict(ldy=10), "apart"), (combine, dict(y=B), "overlaps"), (combine, dict(pos=None), "null"),
+    (experts, dict(type=F32), "16-bit"), (experts, dict(X=2000), "experts"), (experts, dict(offsets=None), "null"), (experts, dict(block=-8), "negative stride"),
+    (experts, dict(ldy=31), "apart"), (experts, dict(ldx=-64), "negative stride"), (experts, dict(ys=B), "overlaps"), (experts, dict(rows=-1), "negative"), (experts, dict(F=1 << 31), "too large"),
     (experts, dict(w=None), "null"),
     (grad_w, dict(out=F16), "32 bits"), (grad_w, dict(block=100), "overlap"), (grad_w, dict(dw=C), "overlaps"), (grad_w, dict(ldw=10, block=4096), "apart"),
 ]
