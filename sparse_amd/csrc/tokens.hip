@@ -176,7 +176,7 @@ struct GradPlan {
     items = c.take<int32_t>(n);
     keys2 = small ? nullptr : c.take<uint32_t>(n);
     items2 = small ? nullptr : c.take<int32_t>(n);
-    hist = small ? nullptr : c.take<int>((int64_t)split.groups << bits);
+    hist = n <= kSelfIds ? nullptr : c.take<int>((int64_t)split.groups << bits);
     named = c.take<uint8_t>(cdiv(V, 4) * 4);
     part = c.take<float>(g.chunks > 1 ? g.chunks * 2 * g.segs * kWave * per : 0);
     bytes = c.used;
@@ -202,6 +202,8 @@ int order_ids(futhark_context *ctx, hipStream_t stream, const I *ids, const Grad
     return 0;
   }
   const int bins = 1 << p.bits, mask = bins - 1;
+  const bool self = n <= kSelfIds;
+  const int *hist = self ? nullptr : p.hist;
   for (int k = 0; k < p.passes; k++) {
     const bool to_first = (p.passes - 1 - k) % 2 == 0;
     PassOut o = {};
@@ -210,15 +212,17 @@ int order_ids(futhark_context *ctx, hipStream_t stream, const I *ids, const Grad
     if (k == 0) {
       const Digits<1, I> d = {ids, nullptr, p.g.n, p.g.V, 0, mask};
       o.named = named;
-      TOK_LAUNCH(ctx, (digit_count_kernel<1, I>), p.split.groups, kSplitThreads, stream, d, p.split.per_group, bins, p.hist,
-                 (uint32_t *)named, named ? cdiv(p.g.V, 4) : 0);
-      TOK_LAUNCH(ctx, (digit_place_kernel<1, I>), p.split.groups, kSplitThreads, stream, d, p.split.per_group, bins, p.bits, (const int *)p.hist, o);
+      if (!self)
+        TOK_LAUNCH(ctx, (digit_count_kernel<1, I>), p.split.groups, kSplitThreads, stream, d, p.split.per_group, bins, p.hist,
+                   (uint32_t *)named, named ? cdiv(p.g.V, 4) : 0);
+      TOK_LAUNCH(ctx, (digit_place_kernel<1, I>), p.split.groups, kSplitThreads, stream, d, p.split.per_group, bins, p.bits, hist, o);
     } else {
       o.items_in = to_first ? p.items2 : p.items;
       const Digits<2, I> d = {nullptr, to_first ? p.keys2 : p.keys, p.g.n, p.g.V, k * p.bits, mask};
-      TOK_LAUNCH(ctx, (digit_count_kernel<2, I>), p.split.groups, kSplitThreads, stream, d, p.split.per_group, bins, p.hist,
-                 (uint32_t *)nullptr, (int64_t)0);
-      TOK_LAUNCH(ctx, (digit_place_kernel<2, I>), p.split.groups, kSplitThreads, stream, d, p.split.per_group, bins, p.bits, (const int *)p.hist, o);
+      if (!self)
+        TOK_LAUNCH(ctx, (digit_count_kernel<2, I>), p.split.groups, kSplitThreads, stream, d, p.split.per_group, bins, p.hist,
+                   (uint32_t *)nullptr, (int64_t)0);
+      TOK_LAUNCH(ctx, (digit_place_kernel<2, I>), p.split.groups, kSplitThreads, stream, d, p.split.per_group, bins, p.bits, hist, o);
     }
   }
   return 0;
@@ -460,7 +464,7 @@ int sparse_amd_tokens_lookup_grad(struct futhark_context *ctx, void *stream, int
 }
 
 int64_t sparse_amd_tokens_route_workspace(int64_t n, int64_t X) {
-  if (n <= kOneGroupChoices || X < 1) return 0;
+  if (n <= kSelfChoices || X < 1) return 0;
   return (Split(n).groups * (X + 1) * (int64_t)sizeof(int) + 255) & ~(int64_t)255;
 }
 
@@ -486,10 +490,12 @@ int sparse_amd_tokens_route(struct futhark_context *ctx, void *stream, const voi
         SAMD_TRY(check_work(ctx, who, work, work_bytes, sparse_amd_tokens_route_workspace(n, X)));
         const Split sp(n);
         const Digits<0, I> d = {(const I *)chosen, nullptr, n, X, 0, 0};
-        TOK_LAUNCH(ctx, (digit_count_kernel<0, I>), sp.groups, kSplitThreads, s, d, sp.per_group, (int)X + 1, (int *)work, (uint32_t *)nullptr, (int64_t)0);
+        const bool self = n <= kSelfChoices;
+        if (!self)
+          TOK_LAUNCH(ctx, (digit_count_kernel<0, I>), sp.groups, kSplitThreads, s, d, sp.per_group, (int)X + 1, (int *)work, (uint32_t *)nullptr, (int64_t)0);
         PassOut o = {};
         o.pos = pos; o.src = src; o.offsets = offsets;
-        TOK_LAUNCH(ctx, (digit_place_kernel<0, I>), sp.groups, kSplitThreads, s, d, sp.per_group, (int)X + 1, bits, (const int *)work, o);
+        TOK_LAUNCH(ctx, (digit_place_kernel<0, I>), sp.groups, kSplitThreads, s, d, sp.per_group, (int)X + 1, bits, self ? (const int *)nullptr : (const int *)work, o);
       }
       return 0;
     });

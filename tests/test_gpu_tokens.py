@@ -138,8 +138,8 @@ def lookup_grad_ref(dy, ids, V, f):
     return z.clone().index_add_(0, at, rows), z.index_add_(0, at, rows.abs()), count[:, None]
 
 
-GRADS = [(1, 1, 1, "uniform"), (1, 5000, 64, "uniform"), (5, 3, 7, "wild"), (100, 40, 65, "skew"), (300, 17, 1001, "uniform"), (1000, 1, 130, "one"), (256, 1, 40, "one"), (256, 9, 72, "skew"), (257, 9, 72, "skew"), (200, 70000, 8, "skew"), (33, 50, 3001, "uniform"), (100, 20000000, 1, "wild"), (2048, 300, 56, "skew"), (2049, 300, 56, "skew"),
-         (1025, 700, 520, "wild"), (4097, 300000, 24, "skew"), (8192, 50, 96, "skew"), (8193, 1000, 40, "skew"), (16384, 1000, 40, "skew"), (16385, 9000, 24, "skew"), (20000, 131072, 64, "skew"),
+GRADS = [(1, 1, 1, "uniform"), (1, 5000, 64, "uniform"), (5, 3, 7, "wild"), (100, 40, 65, "skew"), (300, 17, 1001, "uniform"), (1000, 1, 130, "one"), (256, 1, 40, "one"), (256, 9, 72, "skew"), (257, 9, 72, "skew"), (200, 70000, 8, "skew"), (33, 50, 3001, "uniform"), (100, 20000000, 1, "wild"), (2048, 300, 56, "skew"), (2049, 300, 56, "skew"), (5000, 70, 33, "wild"), (3000, 5000000, 2, "skew"),
+         (1025, 700, 520, "wild"), (4096, 300000, 24, "skew"), (4097, 300000, 24, "skew"), (8192, 50, 96, "skew"), (8193, 1000, 40, "skew"), (16384, 1000, 40, "skew"), (16385, 9000, 24, "skew"), (20000, 131072, 64, "skew"),
          (30000, 3, 33, "one"), (600000, 2000, 8, "uniform"), (9000, 100, 16, "none"), (70, 9, 12, "none"), (9000, 3000000, 1, "wild"),
          (2048, 64, 4096, "uniform")]
 
@@ -220,7 +220,7 @@ def route_ref(c, X):
     return pos.reshape(c.shape), src, np.searchsorted(key[order], np.arange(X + 1))
 
 
-ROUTES = [(0, 2, 4), (1, 1, 1), (1, 8, 64), (64, 4, 1024), (65, 4, 3), (256, 4, 256), (1000, 8, 17), (1025, 8, 1000), (4096, 2, 8), (4097, 2, 8), (8192, 2, 64), (8193, 2, 1000),
+ROUTES = [(0, 2, 4), (1, 1, 1), (1, 8, 64), (64, 4, 1024), (65, 4, 3), (256, 4, 256), (1000, 8, 17), (1025, 8, 1000), (4096, 2, 8), (4097, 2, 8), (8192, 2, 64), (8193, 2, 1000), (5461, 3, 1024),
           (30001, 3, 128), (150000, 4, 1024), (600000, 2, 5)]
 
 

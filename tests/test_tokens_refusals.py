@@ -114,7 +114,7 @@ def test_workspaces():
     assert f(BF16, 10000, 1000, 64) > 8 * 10000 + 2 * (10000 // 32) * 64 * 4
     g = L.sparse_amd_tokens_route_workspace
     g.argtypes, g.restype = (I64, I64), I64
-    assert g(4096, 1024) == 0 and g(4097, 1024) >= 4 * 1025 and g(1 << 30, 1024) <= 2 << 20
+    assert g(8192, 1024) == 0 and g(8193, 1024) >= 4 * 1025 and g(1 << 30, 1024) <= 2 << 20
 
 
 def test_the_python_side_refuses_what_is_not_on_the_device():
