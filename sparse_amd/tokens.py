@@ -26,6 +26,7 @@ call is one entry of include/sparse_amd.h, group (7), where the formulas stand. 
 Arguments that do not fit (type, shape, device, overlap) raise SparseError before anything is launched.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -94,53 +95,66 @@ class mk_tokens:
             f = getattr(L, "sparse_amd_tokens_" + name)
             f.argtypes = types
             setattr(self, "_c_" + name, f)
-        self._c_grad_work = L.sparse_amd_tokens_lookup_grad_workspace
-        self._c_grad_work.argtypes, self._c_grad_work.restype = (_INT, _I64, _I64, _I64), _I64
-        self._c_route_work = L.sparse_amd_tokens_route_workspace
-        self._c_route_work.argtypes, self._c_route_work.restype = (_I64, _I64), _I64
+        # how much a workspace takes depends on the sizes alone: asked once for each of the last ones
+        f = L.sparse_amd_tokens_lookup_grad_workspace
+        f.argtypes, f.restype = (_INT, _I64, _I64, _I64), _I64
+        self._c_grad_work = functools.lru_cache(256)(f)
+        f = L.sparse_amd_tokens_route_workspace
+        f.argtypes, f.restype = (_I64, _I64), _I64
+        self._c_route_work = functools.lru_cache(256)(f)
 
-    # ---- arguments
-    def _tensor(self, a, name, dtypes, dims):
-        """(address, dtype) of an argument that is a tensor of one of these types and so many dimensions, on the device."""
-        if not isinstance(a, torch.Tensor) or not a.is_cuda or a.get_device() != self._dev:
+    # ---- arguments: what fits is taken with a handful of attribute reads, since a small call costs as much as they do; what
+    # does not is looked at again for the message
+    def _refuse(self, a, name, dtypes, why):
+        if not isinstance(a, torch.Tensor) or a.get_device() != self._dev:
             raise SparseError("%s: expected a tensor on cuda:%d" % (name, self._dev))
         if a.dtype not in dtypes:
             raise SparseError("%s: expected %s, got %s" % (name, " or ".join(str(d) for d in dtypes), a.dtype))
-        if dims is not None and a.dim() != dims:
-            raise SparseError("%s: expected %d dimensions, got %d" % (name, dims, a.dim()))
-        return a.data_ptr()
+        raise SparseError("%s: %s" % (name, why))
 
-    def _panel(self, a, name, rows=None, cols=None, dtypes=None):
+    def _panel(self, a, name, rows=None, cols=None, dtype=None):
         """(address, row stride, rows, columns) of a 2-d panel with contiguous rows."""
-        p = self._tensor(a, name, dtypes or (self._dtype,), 2)
+        dtype = dtype or self._dtype
+        if not isinstance(a, torch.Tensor) or a.dtype is not dtype or a.get_device() != self._dev:
+            self._refuse(a, name, (dtype,), "")
+        if a.dim() != 2:
+            self._refuse(a, name, (dtype,), "expected 2 dimensions, got %d" % a.dim())
         n, d = a.shape
-        if (rows is not None and n != rows) or (cols is not None and d != cols):
-            raise SparseError("%s: expected %s x %s, got %d x %d" % (name, "any" if rows is None else rows, "any" if cols is None else cols, n, d))
         ld, step = a.stride()
+        if (rows is not None and n != rows) or (cols is not None and d != cols):
+            self._refuse(a, name, (dtype,), "expected %s x %s, got %d x %d" % ("any" if rows is None else rows, "any" if cols is None else cols, n, d))
         if step != 1 and d > 1:
-            raise SparseError("%s: the elements of a row are not side by side" % name)
-        return p, ld if n > 1 else max(ld, d), n, d
+            self._refuse(a, name, (dtype,), "the elements of a row are not side by side")
+        return a.data_ptr(), ld if n > 1 or ld > d else d, n, d
 
-    def _flat(self, a, name, dtypes, shape=None):
-        """Address of a contiguous tensor (of that shape)."""
-        p = self._tensor(a, name, dtypes, None)
-        if shape is not None and a.shape != shape:
+    def _floats(self, a, name, shape):
+        """Address of a contiguous float32 tensor of this shape."""
+        if not isinstance(a, torch.Tensor) or a.dtype is not torch.float32 or a.get_device() != self._dev:
+            self._refuse(a, name, (torch.float32,), "")
+        if a.shape != shape:
             raise SparseError("%s: expected shape %s, got %s" % (name, tuple(shape), tuple(a.shape)))
         if not a.is_contiguous():
             raise SparseError("%s: not contiguous" % name)
-        return p
+        return a.data_ptr()
 
     def _ids(self, a, name):
-        p = self._flat(a, name, (torch.int64, torch.int32))
-        return p, 64 if a.dtype == torch.int64 else 32, a.numel()
+        """(address, bits, count) of contiguous indices."""
+        if not isinstance(a, torch.Tensor) or a.get_device() != self._dev:
+            self._refuse(a, name, (torch.int64, torch.int32), "")
+        bits = 64 if a.dtype is torch.int64 else 32 if a.dtype is torch.int32 else 0
+        if not bits:
+            self._refuse(a, name, (torch.int64, torch.int32), "")
+        if not a.is_contiguous():
+            raise SparseError("%s: not contiguous" % name)
+        return a.data_ptr(), bits, a.numel()
 
     def _out(self, out, name, rows, cols, dtype=None):
         """The result's panel: `out`, checked, or a new one."""
         dtype = dtype or self._dtype
         if out is None:
             out = torch.empty((rows, cols), dtype=dtype, device=self._device)
-            return out, out.data_ptr(), max(cols, 1)
-        p, ld, _, _ = self._panel(out, name, rows, cols, (dtype,))
+            return out, out.data_ptr(), cols or 1
+        p, ld, _, _ = self._panel(out, name, rows, cols, dtype)
         return out, p, ld
 
     def _sum_type(self, out, dtype):
@@ -150,9 +164,10 @@ class mk_tokens:
         return dtype, self._code if dtype == self._dtype else 0
 
     def _call(self, f, *args):
-        if not self.ctx.h:
+        h = self.ctx.h
+        if not h:
             raise SparseError("the context is closed")
-        if f(self.ctx.h, _current_stream(self._dev), *args):
+        if f(h, _current_stream(self._dev), *args):
             raise SparseError(self.ctx.error() or "entry point failed")
 
     def _scratch(self, size):
@@ -176,7 +191,7 @@ class mk_tokens:
         id, or None (ones).  `out`: a panel [ids.numel(), D] to write instead of a new tensor (returned as it is)."""
         e, lde, V, D = self._panel(E, "E")
         i, bits, n = self._ids(ids, "ids")
-        f = self._flat(vals, "vals", (torch.float32,), ids.shape) if vals is not None else None
+        f = self._floats(vals, "vals", ids.shape) if vals is not None else None
         y, p, ldy = self._out(out, "out", n, D)
         self._call(self._c_lookup, self._code, p, ldy, e, V, D, lde, i, bits, n, f, scale)
         return y if out is not None or ids.dim() == 1 else y.view(*ids.shape, D)
@@ -191,7 +206,7 @@ class mk_tokens:
         if V < 0:
             raise SparseError("lookup_grad: %d rows" % V)
         g, ldg, _, D = self._panel(self._as_rows(dy, ids), "dy", rows=n)
-        f = self._flat(vals, "vals", (torch.float32,), ids.shape) if vals is not None else None
+        f = self._floats(vals, "vals", ids.shape) if vals is not None else None
         if accumulate and out is None:
             raise SparseError("lookup_grad: accumulate needs `out`")
         dtype, code = self._sum_type(out, dtype)
@@ -231,7 +246,7 @@ class mk_tokens:
         return r
 
     def _weights(self, w, r):
-        return self._flat(w, "weights", (torch.float32,), (r.tokens, r.K)) if w is not None else None
+        return self._floats(w, "weights", (r.tokens, r.K)) if w is not None else None
 
     def dispatch(self, x, r, weights=None, out=None):
         """xs[pos[t, j]] = weights[t, j] * x[t]: [slots, D], rows in the order of their experts."""
@@ -268,16 +283,20 @@ class mk_tokens:
         return dys, dw
 
     # ---- one dense block per expert
-    def _blocks(self, W, name, X, dtypes=None):
+    def _blocks(self, W, name, X, dtype=None):
         """(address, F, D, row stride, block stride) of [X, F, D] with contiguous rows."""
-        p = self._tensor(W, name, dtypes or (self._dtype,), 3)
+        dtype = dtype or self._dtype
+        if not isinstance(W, torch.Tensor) or W.dtype is not dtype or W.get_device() != self._dev:
+            self._refuse(W, name, (dtype,), "")
+        if W.dim() != 3:
+            self._refuse(W, name, (dtype,), "expected 3 dimensions, got %d" % W.dim())
         x, F, D = W.shape
         if x != X:
             raise SparseError("%s: %d blocks for %d experts" % (name, x, X))
         block, ld, step = W.stride()
         if step != 1 and D > 1:
             raise SparseError("%s: the elements of a row are not side by side" % name)
-        return p, F, D, ld if F > 1 else max(ld, D), block
+        return W.data_ptr(), F, D, ld if F > 1 or ld > D else D, block
 
     def experts(self, xs, W, r, out=None):
         """ys[p] = W[e] xs[p] for every expert e's places p: [slots, F] from xs[slots, D], W[X, F, D]."""
@@ -308,7 +327,7 @@ class mk_tokens:
         dtype, code = self._sum_type(out, dtype)
         if out is None:
             out = torch.empty((r.X, F, D), dtype=dtype, device=self._device)
-        w, f, d, ldw, block = self._blocks(out, "out", r.X, (dtype,))
+        w, f, d, ldw, block = self._blocks(out, "out", r.X, dtype)
         if (f, d) != (F, D):
             raise SparseError("out: expected blocks of %d x %d, got %d x %d" % (F, D, f, d))
         self._call(self._c_experts_grad_w, self._code, code, int(accumulate), w, r.X, F, D, ldw, block, g, ldg, a, lda, n, r._offsets)
