@@ -38,7 +38,8 @@ int entry(futhark_context *ctx, F body) {
   if (!ctx) return 1;
   try {
     OnDevice on(ctx);
-    return body();
+    const int rc = body();
+    return rc ? rc : need_device(ctx);
   } catch (...) {
     return 1;
   }
