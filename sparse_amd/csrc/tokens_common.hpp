@@ -6,6 +6,7 @@
 #pragma once
 
 #include "common.hpp"
+#include "scan.hpp"
 
 namespace samd {
 namespace tok {
@@ -14,8 +15,8 @@ using bf16 = __bf16;
 using f16 = _Float16;
 
 constexpr int kWave = 64;
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
+constexpr int kThreads = kBlock;  // kWaves waves
+static_assert(kThreads == kWaves * kWave, "a workgroup is a whole number of waves");
 
 template <class T>
 constexpr int kPer = 16 / (int)sizeof(T);  // elements of a 16-byte piece

@@ -204,49 +204,29 @@ __device__ __forceinline__ int place_of(int id, int tiles) {
   return id / kXcds < per && t < tiles ? t : -1;
 }
 
-// How many m-tiles the experts have in all.
-__device__ __forceinline__ int count_tiles(const int32_t *offsets, int X, int64_t rows, int bm) {
-  int tiles = 0;
-  for (int e = lane_id(); e < X; e += kWave) {
-    const int64_t a = clamped(offsets, e, rows), b = clamped(offsets, e + 1, rows);
-    tiles += b > a ? (int)((b - a + bm - 1) / bm) : 0;
+// The experts' m-tiles, 64 experts at a time: lane l has those of expert e0 + l, counted up to and with it.
+struct TileCounts {
+  int32_t a, b;   // the expert's rows
+  int upto;
+  __device__ __forceinline__ TileCounts(const int32_t *offsets, int e0, int X, int64_t rows, int bm) {
+    const int e = e0 + lane_id();
+    a = b = 0;
+    if (e < X) {
+      a = (int32_t)clamped(offsets, e, rows);
+      b = (int32_t)clamped(offsets, e + 1, rows);
+    }
+    upto = (int)wave_inclusive_add_dpp(b > a ? (uint32_t)(b - a + bm - 1) / (uint32_t)bm : 0u);
   }
-#pragma unroll
-  for (int d = kWave / 2; d > 0; d >>= 1) tiles += __shfl_xor(tiles, d, kWave);
-  return __builtin_amdgcn_readfirstlane(tiles);
-}
-
-// The expert whose m-tile `tile` is, counted over all experts; its first row and the expert's last.  False: there is none.
-__device__ __forceinline__ bool find_tile(const int32_t *offsets, int X, int64_t rows, int bm, int tile, int *e, int64_t *r0, int64_t *r1) {
-  const int l = lane_id();
-  int before = 0;
-  for (int e0 = 0; e0 < X; e0 += kWave) {
-    const int mine = e0 + l;
-    int64_t a = 0, b = 0;
-    if (mine < X) {
-      a = clamped(offsets, mine, rows);
-      b = clamped(offsets, mine + 1, rows);
-    }
-    const int tiles = b > a ? (int)((b - a + bm - 1) / bm) : 0;
-    int s = tiles;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const int o = __shfl_up(s, d, kWave);
-      if (l >= d) s += o;
-    }
-    const uint64_t past = __ballot(before + s > tile);
-    if (past) {
-      const int w = __ffsll((unsigned long long)past) - 1;
-      const int first = before + __builtin_amdgcn_readlane(s - tiles, w);
-      *e = e0 + w;
-      *r0 = same(__shfl(a, w, kWave)) + (int64_t)(tile - first) * bm;
-      *r1 = same(__shfl(b, w, kWave));
-      return true;
-    }
-    before += __builtin_amdgcn_readlane(s, kWave - 1);
+  __device__ __forceinline__ int all() const { return __builtin_amdgcn_readlane(upto, kWave - 1); }
+  // The expert (of these 64) whose tile the `tile`-th of these is; its first row in the tile, and the expert's last.
+  __device__ __forceinline__ int find(int tile, int bm, int64_t *r0, int64_t *r1) const {
+    const int w = __builtin_ctzll(__ballot(upto > tile));
+    const int before = w > 0 ? __builtin_amdgcn_readlane(upto, w - 1) : 0;
+    *r0 = __builtin_amdgcn_readlane(a, w) + (int64_t)(tile - before) * bm;
+    *r1 = __builtin_amdgcn_readlane(b, w);
+    return w;
   }
-  return false;
-}
+};
 
 template <class T, class TO, bool ADD>
 __device__ __forceinline__ void store_four(TO *p, const typename Mfma<T>::Acc &a, int64_t left) {
@@ -313,7 +293,10 @@ __device__ __forceinline__ bool place_product(int *e, int64_t *m0, int64_t *n0, 
     *m_end = g.M;
     return true;
   }
-  const int m_tiles = count_tiles(offsets, g.X, g.rows, BM), tiles = m_tiles * g.n_tiles;
+  const TileCounts first(offsets, 0, g.X, g.rows, BM);  // all there are, as a rule
+  int m_tiles = first.all();
+  for (int e0 = kWave; e0 < g.X; e0 += kWave) m_tiles += TileCounts(offsets, e0, g.X, g.rows, BM).all();
+  const int tiles = m_tiles * g.n_tiles;
   const int rest = tiles % g.split, whole = g.split > 1 && 2 * rest <= g.split ? tiles - rest : tiles;
   const int own = (whole + kXcds - 1) / kXcds * kXcds;  // workgroups of the whole tiles
   int t;
@@ -327,7 +310,19 @@ __device__ __forceinline__ bool place_product(int *e, int64_t *m0, int64_t *n0, 
     if (t >= tiles) return false;
   }
   tile_at(t, m_tiles, g.n_tiles, &m, &n);
-  if (!find_tile(offsets, g.X, g.rows, BM, m, e, m0, m_end)) return false;
+  if (m < first.all()) {
+    *e = first.find(m, BM, m0, m_end);
+  } else {
+    m -= first.all();
+    for (int e0 = kWave; e0 < g.X; e0 += kWave) {
+      const TileCounts more(offsets, e0, g.X, g.rows, BM);
+      if (m < more.all()) {
+        *e = e0 + more.find(m, BM, m0, m_end);
+        break;
+      }
+      m -= more.all();
+    }
+  }
   *n0 = (int64_t)n * BN;
   if (*quarter >= 0) {
     *m0 += (*quarter >> 1) * (BM / 2);

@@ -56,14 +56,8 @@ __device__ __forceinline__ void wave_ranks(const int (&digit)[IPL], int (&rank)[
 // Exclusive scan over the threads of a workgroup of NW waves.
 template <int NW>
 __device__ __forceinline__ int group_scan(int v, int *wave_total, int *total) {
-  const int lane = lane_id();
-  int s = v;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const int o = __shfl_up(s, d, kWave);
-    if (lane >= d) s += o;
-  }
-  if (lane == kWave - 1) wave_total[wave_id()] = s;
+  const int s = (int)wave_inclusive_add_dpp((uint32_t)v);
+  if (lane_id() == kWave - 1) wave_total[wave_id()] = s;
   __syncthreads();
   int before = 0, all = 0;
 #pragma unroll
