@@ -294,9 +294,9 @@ int launch_experts(futhark_context *ctx, const char *who, hipStream_t stream, TO
   }
   blocks = cdiv(blocks, kXcds) * kXcds;
   g.split = 1;
-  if (KIND != kGradW && BM == 256 && BN == 256 && m_tiles * n_tiles > ctx->num_cu) {  // room for the quarters of half a round
+  if (KIND != kGradW && BM == 256 && BN == 256 && m_tiles * n_tiles > ctx->num_cu) {  // room for the halves of half a round
     g.split = ctx->num_cu;
-    blocks += 3 * (cdiv(ctx->num_cu / 2, kXcds) * kXcds) + 2 * kXcds;
+    blocks += cdiv(ctx->num_cu / 2, kXcds) * kXcds + 4 * kXcds;
   }
   SAMD_TRY(check_blocks(ctx, who, blocks));
   g.m_tiles = (int)m_tiles;
@@ -316,26 +316,37 @@ int experts_panels(futhark_context *ctx, const char *who, hipStream_t stream, T 
     if (g.rows <= 48 * g.X) return launch_experts<T, T, KIND, 32, 64, 128, 1, 4, false, false, true>(ctx, who, stream, C, A, B, offsets, g);
     return launch_experts<T, T, KIND, 128, 128, 64, 2, 2, false, false, true>(ctx, who, stream, C, A, B, offsets, g);
   }
-  // The tile whose launch is estimated to end first: whole rounds of the card's 256 CUs, by the rate each tile reaches with
-  // the card full (TFLOP/s, measured on 32 experts of 4096 x 2048).  Small tiles waste fewer rows of a small expert, large
-  // ones read each operand less often: 64 rows an expert, forward: 64 x 256 136 us, 256 x 256 146; 256 rows: 244 and 180.
-  struct { int bm, bn, per_cu, rate; } const tiles[] = {{32, 64, 3, 400}, {64, 256, 2, 600}, {128, 128, 2, 800}, {128, 256, 1, 900}, {256, 256, 1, 1200}};
-  const int64_t used = g.rows < g.X ? g.rows : g.X, mean = cdiv(g.rows, used);
+  // The tile whose launch is estimated to end first: rounds of the card's CUs, at the time that a tile takes for 64 of the
+  // summed index, or one pass over the blocks where no cache holds them, at the rate that a tile's loads reach (a tile that
+  // reads 64 bytes of every row of W is slow at that).  Both were fitted to the times of all five tiles for 4 to 2048 rows
+  // an expert in eight shapes from 2 blocks of 2048 x 512 to 32 of 4096 x 2048, where the choice is 1.4 % behind the fastest
+  // tile on average and 18 % at most (an estimate from rates alone: 9 % and 82 %); in five others, 256 wide to 8192, 3 %.
+  // Small tiles waste fewer rows of a small expert, large ones read each operand less often: 32 experts of 4096 x 2048,
+  // forward, 16 rows each: 32 x 64 98 us, 256 x 256 128; 96 rows: 128 x 128 126, 256 x 256 133, 32 x 64 204; 256 rows: 252,
+  // 170 and 410.
+  struct Cost { int bm, bn; double step, rate; };  // microseconds, TB/s
+  static const Cost forward[] = {{32, 64, 0.22, 5.6}, {64, 256, 0.78, 3.0}, {128, 128, 0.69, 4.8}, {128, 256, 0.93, 3.5}, {256, 256, 1.31, 4.1}};
+  static const Cost grad_x[] = {{32, 64, 0.16, 4.3}, {64, 256, 0.68, 5.2}, {128, 128, 0.64, 4.0}, {128, 256, 1.02, 3.5}, {256, 256, 1.27, 5.0}};
+  const Cost *const tiles = KIND == kForward ? forward : grad_x;
+  const double used = (double)(g.rows < g.X ? g.rows : g.X), mean = (double)g.rows / used, bytes = used * g.N * g.K * sizeof(T);
+  const bool cached = bytes <= (double)((int64_t)256 << 20);  // the card's last cache
   int best = 0;
   double least = 0;
   for (int i = 0; i < 5; i++) {
-    const int64_t count = used * cdiv(mean, tiles[i].bm) * cdiv(g.N, tiles[i].bn);
-    double rounds = (double)cdiv(count, 256 * tiles[i].per_cu);
-    if (i == 4 && count > 256 && count % 256 > 0 && count % 256 <= 128) rounds -= 0.5;  // a last round that is cut into quarters
-    const double t = rounds * tiles[i].per_cu * tiles[i].bm * tiles[i].bn / tiles[i].rate;
+    // an expert's last tile is half full, if it has several
+    const double full = mean / tiles[i].bm + 0.5, count = used * (full > 1 ? full : 1) * (double)cdiv(g.N, tiles[i].bn) / ctx->num_cu;
+    double rounds = ceil(count);
+    if (i == 4 && rounds > 1 && rounds - count >= 0.5) rounds -= 0.4;  // a last round of half tiles
+    double t = rounds * ((double)g.K / 64) * tiles[i].step;
+    if (!cached && bytes / tiles[i].rate * 1e-6 > t) t = bytes / tiles[i].rate * 1e-6;
     if (i == 0 || t < least) {
       best = i;
       least = t;
     }
   }
-  // weights that the card's last cache (256 MiB) cannot hold until the next call are read past it where a block is read
-  // once: 32 blocks of 4096 x 2048, 110 -> 95 us; 8 of them, which it holds, 22 -> 31
-  const bool once = mean <= tiles[best].bm && used * g.blockB * (int64_t)sizeof(T) > ((int64_t)256 << 20);
+  // weights that no cache can hold until the next call are read past it where nearly every block is read once: 32 blocks
+  // of 4096 x 2048, 110 -> 95 us; 8 of them, which it holds, 22 -> 31; 128 of 2048 x 768 where a few are read twice, 101 -> 146
+  const bool once = 4 * mean <= 3 * tiles[best].bm && !cached;
   switch (best) {
     case 0:
       return once ? launch_experts<T, T, KIND, 32, 64, 64, 1, 4, false, true>(ctx, who, stream, C, A, B, offsets, g)
@@ -344,8 +355,8 @@ int experts_panels(futhark_context *ctx, const char *who, hipStream_t stream, T 
       return once ? launch_experts<T, T, KIND, 64, 256, 32, 1, 4, false, true>(ctx, who, stream, C, A, B, offsets, g)
                   : launch_experts<T, T, KIND, 64, 256, 32, 1, 4, false>(ctx, who, stream, C, A, B, offsets, g);
     case 2: return launch_experts<T, T, KIND, 128, 128, 32, 2, 2, false>(ctx, who, stream, C, A, B, offsets, g);
-    case 3: return launch_experts<T, T, KIND, 128, 256, 32, 2, 4, false>(ctx, who, stream, C, A, B, offsets, g);
-    default: return launch_experts<T, T, KIND, 256, 256, 32, 2, 4, false>(ctx, who, stream, C, A, B, offsets, g);
+    case 3: return launch_experts<T, T, KIND, 128, 256, 64, 2, 4, false>(ctx, who, stream, C, A, B, offsets, g);
+    default: return launch_experts<T, T, KIND, 256, 256, 64, 2, 4, false>(ctx, who, stream, C, A, B, offsets, g);
   }
 }
 
@@ -358,7 +369,7 @@ int experts_weights(futhark_context *ctx, const char *who, hipStream_t stream, T
   }
   // as above: tiles enough for every CU to have a large one, and work in them: with few rows a tile is all writing, and two
   // small ones on a CU overlap it better (16 rows an expert: 145 us against 150)
-  if (g.X * cdiv(g.M, 256) * cdiv(g.N, 256) >= 256 && g.rows > 64 * g.X) return launch_experts<T, TO, kGradW, 256, 256, 32, 2, 4, ADD>(ctx, who, stream, C, A, B, offsets, g);
+  if (g.X * cdiv(g.M, 256) * cdiv(g.N, 256) >= 256 && g.rows > 64 * g.X) return launch_experts<T, TO, kGradW, 256, 256, 64, 2, 4, ADD>(ctx, who, stream, C, A, B, offsets, g);
   return launch_experts<T, TO, kGradW, 128, 128, 32, 2, 2, ADD>(ctx, who, stream, C, A, B, offsets, g);
 }
 

@@ -6,13 +6,16 @@
 //   kGradW     dW[e][f, d] = sum_r dys[r, f] xs[r, d]          (both have it down their rows)
 //
 // One workgroup computes a BM x BN tile of one expert's result; sums are in 32 bits (v_mfma_f32_16x16x32) and rounded
-// once.  A step takes 64 of the summed index: each operand's 64-deep slice goes from memory to LDS without passing
-// through registers (buffer_load ... lds, 16 bytes a lane), one step ahead of the products, in two buffers with one
-// barrier a step.  The buffer descriptor ends at the expert's last row, so what a ragged tile would read beyond it is
-// zero and costs no memory access.
+// once.  A step takes 32, 64 or 128 of the summed index: each operand's slice of it goes from memory to LDS without passing
+// through registers (buffer_load ... lds, 16 bytes a lane), some steps ahead of the products.  The buffer descriptor ends
+// at the expert's last row, so what a ragged tile would read beyond it is zero and costs no memory access.
 //
-// LDS layouts.  "Lying" operands (summed index side by side): row r is 128 bytes, its eight 16-byte chunks permuted by
-// c ^ (r & 7); a fragment is one ds_read_b128.  "Standing" operands (summed index down the rows): row k is R elements,
+// What bounds it: with few rows an expert the blocks' bytes (32 blocks of 4096 x 2048: 98 us, 5.5 TB/s), with many the
+// matrix cores' clock under power: 2048 rows each, 1220 TFLOP/s forward and 1140 for the gradient by xs, where a large
+// library product reaches 1430 to 1520.
+//
+// LDS layouts.  "Lying" operands (summed index side by side): row r is a step's slice, its 16-byte chunks permuted by a
+// function of r; a fragment is one ds_read_b128.  "Standing" operands (summed index down the rows): row k is R elements,
 // its 32-byte units permuted by a function of k; a fragment is two ds_read_b64_tr_b16, which hand a lane four k of one
 // column.  Both permutations spread every group of lanes that is served at once over all 64 banks.  They are applied to
 // the addresses the loads read from, since a load to LDS writes its 64 lanes side by side.
@@ -250,37 +253,45 @@ __device__ __forceinline__ void arrived() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// A tile's operands: rows m0 .. and columns n0 .. of expert e's result, which ends with row m_end.
-template <int KIND, class T, class TO, class TA, class TB>
-__device__ __forceinline__ int64_t operands(TA &ta, TB &tb, TO *&out, int e, int64_t m0, int64_t n0, int64_t m_end, TO *C, const T *A, const T *B,
-                                            const int32_t *offsets, const ProductShape &g) {
-  if (KIND == kGradW) {
-    const int64_t ra = clamped(offsets, e, g.rows), rb = clamped(offsets, e + 1, g.rows), summed = same(rb > ra ? rb - ra : 0);
-    ta.init(A + ra * g.ldA + m0, g.ldA, summed ? (summed - 1) * g.ldA + g.M - m0 : 0, summed, g.M - m0);
-    tb.init(B + ra * g.ldB + n0, g.ldB, summed ? (summed - 1) * g.ldB + g.N - n0 : 0, summed, g.N - n0);
-    out = C + (int64_t)e * g.blockC;
-    return summed;
-  }
-  ta.init(A + m0 * g.ldA, g.ldA, (m_end - m0 - 1) * g.ldA + g.K, g.K, m_end - m0);
-  const T *w = B + (int64_t)e * g.blockB;
-  if (KIND == kForward)
-    tb.init(w + n0 * g.ldB, g.ldB, (g.N - n0 - 1) * g.ldB + g.K, g.K, g.N - n0);
+// The operands of a tile whose rows begin at m0 and columns at n0 of expert e's result, which ends with row m_end.
+template <int KIND, class T, class TA>
+__device__ __forceinline__ void operand_a(TA &ta, int e, int64_t m0, int64_t m_end, int64_t summed, const T *A, const int32_t *offsets, const ProductShape &g) {
+  if (KIND == kGradW)
+    ta.init(A + clamped(offsets, e, g.rows) * g.ldA + m0, g.ldA, summed ? (summed - 1) * g.ldA + g.M - m0 : 0, summed, g.M - m0);
   else
-    tb.init(w + n0, g.ldB, (g.K - 1) * g.ldB + g.N - n0, g.K, g.N - n0);
-  out = C;
-  return g.K;
+    ta.init(A + m0 * g.ldA, g.ldA, (m_end - m0 - 1) * g.ldA + g.K, g.K, m_end - m0);
 }
+template <int KIND, class T, class TB>
+__device__ __forceinline__ void operand_b(TB &tb, int e, int64_t n0, int64_t summed, const T *B, const int32_t *offsets, const ProductShape &g) {
+  if (KIND == kGradW)
+    tb.init(B + clamped(offsets, e, g.rows) * g.ldB + n0, g.ldB, summed ? (summed - 1) * g.ldB + g.N - n0 : 0, summed, g.N - n0);
+  else if (KIND == kForward)
+    tb.init(B + (int64_t)e * g.blockB + n0 * g.ldB, g.ldB, (g.N - n0 - 1) * g.ldB + g.K, g.K, g.N - n0);
+  else
+    tb.init(B + (int64_t)e * g.blockB + n0, g.ldB, (g.K - 1) * g.ldB + g.N - n0, g.K, g.N - n0);
+}
+// How long its sums are, and where its result goes.
+template <int KIND>
+__device__ __forceinline__ int64_t sum_length(int e, const int32_t *offsets, const ProductShape &g) {
+  if (KIND != kGradW) return g.K;
+  const int64_t ra = clamped(offsets, e, g.rows), rb = clamped(offsets, e + 1, g.rows);
+  return same(rb > ra ? rb - ra : 0);
+}
+template <int KIND, class TO>
+__device__ __forceinline__ TO *result_of(TO *C, int e, const ProductShape &g) { return KIND == kGradW ? C + (int64_t)e * g.blockC : C; }
 
 // Where the workgroup's tile is.  False: it has none.
 //
 // A last round of a few tiles of 256 x 256 would leave most CUs idle for as long as any other: if it fills half of them or
-// fewer (g.split: the launch has workgroups enough) each of its tiles is cut into four of 128 x 128; *quarter = which, or -1.
+// fewer (g.split: the launch has workgroups enough) each of its tiles is cut into its upper and its lower rows; *half =
+// which, or -1.  (73 tiles after 256, forward: 262 us whole, 252 in halves, 272 in quarters; in the gradient by xs 301, 286,
+// 308.)
 template <int KIND, int BM, int BN>
-__device__ __forceinline__ bool place_product(int *e, int64_t *m0, int64_t *n0, int64_t *m_end, int *quarter, const int32_t *offsets,
+__device__ __forceinline__ bool place_product(int *e, int64_t *m0, int64_t *n0, int64_t *m_end, int *half, const int32_t *offsets,
                                               const ProductShape &g) {
   const int id = (int)blockIdx.x;
   int m, n;
-  *quarter = -1;
+  *half = -1;
   if (KIND == kGradW) {
     // block after block of dW, each dealt to all dies: the blocks' costs differ with their experts' rows
     const int per = (g.m_tiles * g.n_tiles + kXcds - 1) / kXcds * kXcds;
@@ -304,9 +315,9 @@ __device__ __forceinline__ bool place_product(int *e, int64_t *m0, int64_t *n0, 
     t = place_of(id, whole);
     if (t < 0) return false;
   } else {
-    const int q = id - own;  // the quarters of a tile go to one die
-    t = whole + q / (4 * kXcds) * kXcds + q % kXcds;
-    *quarter = q / kXcds % 4;
+    const int q = id - own;  // the halves of a tile go to one die
+    t = whole + q / (2 * kXcds) * kXcds + q % kXcds;
+    *half = q / kXcds % 2;
     if (t >= tiles) return false;
   }
   tile_at(t, m_tiles, g.n_tiles, &m, &n);
@@ -324,12 +335,8 @@ __device__ __forceinline__ bool place_product(int *e, int64_t *m0, int64_t *n0, 
     }
   }
   *n0 = (int64_t)n * BN;
-  if (*quarter >= 0) {
-    *m0 += (*quarter >> 1) * (BM / 2);
-    *n0 += (*quarter & 1) * (BN / 2);
-    return *m0 < *m_end && *n0 < g.N;
-  }
-  return true;
+  if (*half == 1) *m0 += BM / 2;
+  return *m0 < *m_end;
 }
 
 // Sums in 32 bits, or added to what is there: every lane writes the four neighbouring columns that it holds.
@@ -399,12 +406,14 @@ __global__ __launch_bounds__(WM *WN *kWave) void experts_any_kernel(TO *__restri
   __shared__ __align__(128) T sb[2][BN * DEPTH];
   TA ta;
   TB tb;
-  TO *out;
-  int e, quarter;
+  int e, half;
   int64_t m0, n0, m_end;
-  if (!place_product<KIND, BM, BN>(&e, &m0, &n0, &m_end, &quarter, offsets, g)) return;
-  const int64_t summed = operands<KIND>(ta, tb, out, e, m0, n0, m_end, C, A, B, offsets, g);
+  if (!place_product<KIND, BM, BN>(&e, &m0, &n0, &m_end, &half, offsets, g)) return;
+  const int64_t summed = sum_length<KIND>(e, offsets, g);
   if (ADD && summed == 0) return;
+  operand_a<KIND>(ta, e, m0, m_end, summed, A, offsets, g);
+  operand_b<KIND>(tb, e, n0, summed, B, offsets, g);
+  TO *const out = result_of<KIND>(C, e, g);
   const int wm = wave_id() / WN, wn = wave_id() % WN;
   Acc acc[NI][MI] = {};
   // the products of the step in buffer SET; the next step goes from registers into the other one
@@ -451,41 +460,36 @@ __global__ __launch_bounds__(WM *WN *kWave) void experts_any_kernel(TO *__restri
   }
 }
 
-// Rows that begin on 16 bytes.  Four stages of LDS, each DEPTH of the summed index: a stage's loads are started three steps
-// before its products.  A step of a wave: read this stage's fragments, start the loads of the stage three on, wait for
-// the fragments and for its own loads of the next stage (not for the later ones: vmcnt counts down in order), barrier, products.
-// Behind the barrier every wave's loads of the next stage are there, and the stage before this one may be overwritten.
-// Loads behind the end of the summed index are started like any others, read nothing and write zeros, so that the
-// number of loads in flight, which the wait counts, is always the same.
-//
-// With eight waves, two on each SIMD, waves 4 to 7 run one barrier behind waves 0 to 3 and every step has a second
-// barrier behind its products: while one wave of a SIMD feeds the matrix cores the other reads LDS, and they change places.
-// A stage is then read half a step later by the second four, still before the barrier behind which it is overwritten.
+// Rows that begin on 16 bytes: loads go to LDS by themselves, some steps ahead of the products.  Loads behind the end of the
+// summed index are started like any others, read nothing and write zeros, so that the number of loads in flight, which a
+// wait for the older ones counts (vmcnt counts down in order), is always the same.
 //
 // ONCE: B is read past the caches, for weights that no cache could hold anyway.
-template <class T>
-struct Stages {  // an array for each stage and operand: what is read from one does not wait for loads into another
-  T *a0, *a1, *a2, *a3, *b0, *b1, *b2, *b3;
-};
 
+// Four waves, two or three workgroups on a CU.  Four stages of LDS, each DEPTH of the summed index: a stage's loads are
+// started three steps before its products.  A step: read this stage's fragments, start the loads of the stage three on,
+// wait for the fragments and for the wave's own loads of the next stage, barrier, products.  Behind the barrier every
+// wave's loads of the next stage are there, and the stage before this one may be overwritten.
 template <class T, class TO, int KIND, int BM, int BN, int DEPTH, int WM, int WN, bool ADD, bool ONCE>
-__device__ __forceinline__ void multiply(const Stages<T> lds, int e, int64_t m0, int64_t n0, int64_t m_end, TO *C, const T *A, const T *B,
-                                         const int32_t *offsets, const ProductShape &g) {
+__device__ __forceinline__ void multiply_small(int e, int64_t m0, int64_t n0, int64_t m_end, TO *C, const T *A, const T *B,
+                                               const int32_t *offsets, const ProductShape &g) {
   constexpr int NT = WM * WN * kWave, S = 4, KK = DEPTH / 32;
   constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
-  constexpr bool kPairs = WM * WN == 8;
   using TA = Tile<T, BM, DEPTH, KIND == kGradW, NT, true>;
   using TB = Tile<T, BN, DEPTH, KIND != kForward, NT, true>;
   using Acc = typename Mfma<T>::Acc;
   using Frag = typename Mfma<T>::Frag;
   constexpr int L = TA::kLoads + TB::kLoads;
-  T *const a0 = lds.a0, *const a1 = lds.a1, *const a2 = lds.a2, *const a3 = lds.a3;
-  T *const b0 = lds.b0, *const b1 = lds.b1, *const b2 = lds.b2, *const b3 = lds.b3;
+  // an array for each stage: what is read from one does not wait for loads into another
+  __shared__ __align__(128) T a0[BM * DEPTH], a1[BM * DEPTH], a2[BM * DEPTH], a3[BM * DEPTH];
+  __shared__ __align__(128) T b0[BN * DEPTH], b1[BN * DEPTH], b2[BN * DEPTH], b3[BN * DEPTH];
   TA ta;
   TB tb;
-  TO *out;
-  const int64_t summed = operands<KIND>(ta, tb, out, e, m0, n0, m_end, C, A, B, offsets, g);
+  const int64_t summed = sum_length<KIND>(e, offsets, g);
   if (ADD && summed == 0) return;
+  operand_a<KIND>(ta, e, m0, m_end, summed, A, offsets, g);
+  operand_b<KIND>(tb, e, n0, summed, B, offsets, g);
+  TO *const out = result_of<KIND>(C, e, g);
   const int wm = wave_id() / WN, wn = wave_id() % WN;
   Acc acc[NI][MI] = {};
   // the products of stage t, which is in sa, sb; na, nb take the stage three on
@@ -504,19 +508,12 @@ __device__ __forceinline__ void multiply(const Stages<T> lds, int e, int64_t m0,
     __builtin_amdgcn_sched_barrier(0);
     arrived<(S - 2) * L>();
     __builtin_amdgcn_sched_barrier(0);
-    if (kPairs) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int kk = 0; kk < KK; kk++)
 #pragma unroll
       for (int j = 0; j < NI; j++)
 #pragma unroll
         for (int i = 0; i < MI; i++) acc[j][i] = Mfma<T>::go(fb[kk][j], fa[kk][i], acc[j][i]);
-    if (kPairs) {
-      __builtin_amdgcn_s_setprio(0);
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_barrier();
-      __builtin_amdgcn_sched_barrier(0);
-    }
   };
   if (summed > 0) {
     ta.start(a0, 0);
@@ -526,8 +523,6 @@ __device__ __forceinline__ void multiply(const Stages<T> lds, int e, int64_t m0,
     ta.start(a2, 2);
     tb.template start<ONCE>(b2, 2);
     arrived<(S - 2) * L>();
-    const bool second = kPairs && wave_id() >= 4;
-    if (second) __builtin_amdgcn_s_barrier();
     for (int64_t k0 = 0; k0 < summed; k0 += S * DEPTH) {  // steps behind the last multiply zeros
       step(a0, b0, a3, b3, 0);
       step(a1, b1, a0, b0, 1);
@@ -536,44 +531,163 @@ __device__ __forceinline__ void multiply(const Stages<T> lds, int e, int64_t m0,
       ta.move(S);
       tb.move(S);
     }
-    if (kPairs && !second) __builtin_amdgcn_s_barrier();  // as many barriers as the others
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // no load may still write to LDS when the workgroup has ended
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may still write to LDS when the workgroup has ended
   }
   if constexpr (std::is_same<T, TO>::value && !ADD) {
     constexpr int part = BM / WM * (BN / WN);  // each wave has a stage's array to itself, one that its part of the tile fits into
     constexpr bool in_a = part <= BM * DEPTH;
-    static_assert(part <= BN * DEPTH && (in_a || !kPairs), "a wave's part of the tile fits into a stage's array");
+    static_assert(WM * WN == 4 && part <= BN * DEPTH, "a wave's part of the tile fits into a stage's array");
     __syncthreads();
     T *const as[4] = {a0, a1, a2, a3}, *const bs[4] = {b0, b1, b2, b3};
     const int w = wave_id();
-    T *mine = bs[0];
+    T *mine = in_a ? as[0] : bs[0];
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
+    for (int k = 1; k < 4; k++)
       if (w == k) mine = in_a ? as[k] : bs[k];
-      if (w == k + 4) mine = bs[k];
-    }
     store_rounded<T, BM, BN, WM, WN>(mine, out, acc, m0, n0, m_end, g);
   } else {
     store_product<T, TO, ADD, BM, BN, WM, WN>(out, acc, m0, n0, m_end, g);
   }
 }
 
+// Eight waves, two on each SIMD, one workgroup on a CU.  LDS holds two steps of 64 of the summed index, so that a row gives
+// whole cache lines; each has three parts that are loaded and given up by themselves: the upper rows, the lower rows, and
+// all columns.  A step is two phases: read the columns' and the upper rows' fragments, multiply; read the lower rows'
+// fragments, multiply.  What a phase has read is overwritten one phase later, with the same part two steps on (the lower
+// rows: a step on, being younger), so every load has two phases of time.
+//
+// Waves 4 to 7 run one barrier behind waves 0 to 3, and every phase has one barrier before its products and one behind:
+// while one wave of a SIMD feeds the matrix cores the other reads LDS and starts loads, and they change places.  A part is
+// then read up to half a phase later by the second four, still before the barrier behind which it is overwritten, and
+// waits count the loads that a barrier later all waves may need.
+//
+// Four stages of 32, as above but in turns, take 64 bytes of a lying operand's row at a time: 16 experts of 4096 x 2048,
+// 1024 rows each, forward: 1202 TFLOP/s, in steps of 64 1291; the other two products, 1295 and 1306, are as fast either way.
+template <class T>
+struct Parts {  // [of the even and the odd steps]; an array each: what is read from one does not wait for loads into another
+  T *up0, *up1, *low0, *low1, *col0, *col1;
+};
+
+template <class T, class TO, int KIND, int BM, int BN, bool ADD>
+__device__ __forceinline__ void multiply_large(const Parts<T> lds, int e, int64_t m0, int64_t n0, int64_t m_end, TO *C, const T *A, const T *B,
+                                               const int32_t *offsets, const ProductShape &g) {
+  constexpr int WM = 2, WN = 4, NT = WM * WN * kWave, DEPTH = 64, KK = 2, HM = BM / 2;
+  constexpr int MI = HM / WM / 16, NI = BN / WN / 16;
+  using TA = Tile<T, HM, DEPTH, KIND == kGradW, NT, true>;
+  using TB = Tile<T, BN, DEPTH, KIND != kForward, NT, true>;
+  using Acc = typename Mfma<T>::Acc;
+  using Frag = typename Mfma<T>::Frag;
+  constexpr int kYounger = TB::kLoads + 2 * TA::kLoads;  // loads started since those that a phase waits for
+  TA up, low;
+  TB col;
+  const int64_t summed = sum_length<KIND>(e, offsets, g);
+  if (ADD && summed == 0) return;
+  operand_a<KIND>(up, e, m0, m_end, summed, A, offsets, g);
+  operand_a<KIND>(low, e, m0 + HM, m_end, summed, A, offsets, g);
+  operand_b<KIND>(col, e, n0, summed, B, offsets, g);
+  TO *const out = result_of<KIND>(C, e, g);
+  const int wm = wave_id() / WN, wn = wave_id() % WN;
+  Acc acc[2][NI][MI] = {};
+  Frag fb[KK][NI];
+  const auto multiply = [&](const Frag(&fa)[KK][MI], Acc(&sum)[NI][MI]) {
+    __builtin_amdgcn_sched_barrier(0);
+    arrived<kYounger>();
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+      for (int j = 0; j < NI; j++)
+#pragma unroll
+        for (int i = 0; i < MI; i++) sum[j][i] = Mfma<T>::go(fb[kk][j], fa[kk][i], sum[j][i]);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // step t (0 or 1, counted from where the tiles were moved to), whose parts are u, l, c; other: where the lower rows of
+  // the next step go
+  const auto step = [&](T *u, const T *l, T *c, T *other, int t) {
+    Frag fa[KK][MI];
+#pragma unroll
+    for (int kk = 0; kk < KK; kk++) {
+#pragma unroll
+      for (int j = 0; j < NI; j++) fb[kk][j] = TB::fragment(c, wn * (BN / WN) + j * 16, kk);
+#pragma unroll
+      for (int i = 0; i < MI; i++) fa[kk][i] = TA::fragment(u, wm * (HM / WM) + i * 16, kk);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    low.start(other, t + 1);
+    multiply(fa, acc[0]);
+#pragma unroll
+    for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+      for (int i = 0; i < MI; i++) fa[kk][i] = TA::fragment(l, wm * (HM / WM) + i * 16, kk);
+    __builtin_amdgcn_sched_barrier(0);
+    col.start(c, t + 2);
+    up.start(u, t + 2);
+    multiply(fa, acc[1]);
+  };
+  if (summed > 0) {
+    col.start(lds.col0, 0);
+    up.start(lds.up0, 0);
+    low.start(lds.low0, 0);
+    col.start(lds.col1, 1);
+    up.start(lds.up1, 1);
+    arrived<kYounger>();
+    const bool second = wave_id() >= 4;
+    if (second) __builtin_amdgcn_s_barrier();
+    for (int64_t k0 = 0; k0 < summed; k0 += 2 * DEPTH) {  // a step behind the last multiplies zeros
+      step(lds.up0, lds.low0, lds.col0, lds.low1, 0);
+      step(lds.up1, lds.low1, lds.col1, lds.low0, 1);
+      up.move(2);
+      low.move(2);
+      col.move(2);
+    }
+    if (!second) __builtin_amdgcn_s_barrier();        // as many barriers as the others
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may still write to LDS when the workgroup has ended
+  }
+  if constexpr (std::is_same<T, TO>::value && !ADD) {
+    constexpr int part = HM / WM * (BN / WN);
+    static_assert(2 * part <= HM * DEPTH, "two waves' parts of half the tile fit into an array of rows");
+    __syncthreads();
+    T *const rows[4] = {lds.up0, lds.up1, lds.low0, lds.low1};
+    const int w = wave_id();
+    T *mine = rows[0];
+#pragma unroll
+    for (int k = 1; k < 4; k++)
+      if (w >> 1 == k) mine = rows[k];
+    mine += (w & 1) * part;
+    store_rounded<T, HM, BN, WM, WN>(mine, out, acc[0], m0, n0, m_end, g);
+    __builtin_amdgcn_wave_barrier();
+    store_rounded<T, HM, BN, WM, WN>(mine, out, acc[1], m0 + HM, n0, m_end, g);
+  } else {
+    store_product<T, TO, ADD, HM, BN, WM, WN>(out, acc[0], m0, n0, m_end, g);
+    store_product<T, TO, ADD, HM, BN, WM, WN>(out, acc[1], m0 + HM, n0, m_end, g);
+  }
+}
+
 template <class T, class TO, int KIND, int BM, int BN, int DEPTH, int WM, int WN, bool ADD, bool ONCE>
 __global__ __launch_bounds__(WM *WN *kWave) void experts_kernel(TO *__restrict__ C, const T *__restrict__ A, const T *__restrict__ B,
                                                                 const int32_t *__restrict__ offsets, ProductShape g) {
-  __shared__ __align__(128) T a0[BM * DEPTH], a1[BM * DEPTH], a2[BM * DEPTH], a3[BM * DEPTH];
-  __shared__ __align__(128) T b0[BN * DEPTH], b1[BN * DEPTH], b2[BN * DEPTH], b3[BN * DEPTH];
-  const Stages<T> lds = {a0, a1, a2, a3, b0, b1, b2, b3};
-  int e, quarter;
+  int e, half;
   int64_t m0, n0, m_end;
-  if (!place_product<KIND, BM, BN>(&e, &m0, &n0, &m_end, &quarter, offsets, g)) return;
-  if constexpr (KIND != kGradW && BM == 256 && BN == 256) {
-    if (quarter >= 0) {
-      multiply<T, TO, KIND, BM / 2, BN / 2, DEPTH, WM, WN, ADD, ONCE>(lds, e, m0, n0, m_end, C, A, B, offsets, g);
-      return;
+  if (!place_product<KIND, BM, BN>(&e, &m0, &n0, &m_end, &half, offsets, g)) return;
+  if constexpr (WM * WN == 4) {
+    multiply_small<T, TO, KIND, BM, BN, DEPTH, WM, WN, ADD, ONCE>(e, m0, n0, m_end, C, A, B, offsets, g);
+  } else {
+    static_assert(WM == 2 && WN == 4 && DEPTH == 64 && !ONCE, "as multiply_large has it");
+    __shared__ __align__(128) T up0[BM / 2 * DEPTH], up1[BM / 2 * DEPTH], low0[BM / 2 * DEPTH], low1[BM / 2 * DEPTH];
+    __shared__ __align__(128) T col0[BN * DEPTH], col1[BN * DEPTH];
+    const Parts<T> lds = {up0, up1, low0, low1, col0, col1};
+    if constexpr (KIND != kGradW && BM == 256 && BN == 256) {
+      if (half >= 0) {
+        multiply_large<T, TO, KIND, BM / 2, BN, ADD>(lds, e, m0, n0, m_end, C, A, B, offsets, g);
+        return;
+      }
     }
+    multiply_large<T, TO, KIND, BM, BN, ADD>(lds, e, m0, n0, m_end, C, A, B, offsets, g);
   }
-  multiply<T, TO, KIND, BM, BN, DEPTH, WM, WN, ADD, ONCE>(lds, e, m0, n0, m_end, C, A, B, offsets, g);
 }
 
 }  // namespace tok
