@@ -317,16 +317,15 @@ int experts_panels(futhark_context *ctx, const char *who, hipStream_t stream, T 
     return launch_experts<T, T, KIND, 128, 128, 64, 2, 2, false, false, true>(ctx, who, stream, C, A, B, offsets, g);
   }
   // The tile whose launch is estimated to end first: rounds of the card's CUs, at the time that a tile takes for 64 of the
-  // summed index, or one pass over the blocks where no cache holds them, at the rate that a tile's loads reach (a tile that
-  // reads 64 bytes of every row of W is slow at that).  Both were fitted to the times of all five tiles for 4 to 2048 rows
-  // an expert in eight shapes from 2 blocks of 2048 x 512 to 32 of 4096 x 2048, where the choice is 1.4 % behind the fastest
-  // tile on average and 18 % at most (an estimate from rates alone: 9 % and 82 %); in five others, 256 wide to 8192, 3 %.
+  // summed index, or one pass over the blocks where no cache holds them, at the rate that a tile's loads reach (64 bytes of
+  // every row of W at a time are slower than whole lines).  Both were fitted to the times of all five tiles for 2 to 2048
+  // rows an expert in eleven shapes from 2 blocks of 2048 x 512 to 32 of 4096 x 2048, where the choice is 1.3 % behind the
+  // fastest tile on average and 29 % at most; in six others, 256 wide to 8192, 2.9 % (from rates alone: 9 % and 82 %).
   // Small tiles waste fewer rows of a small expert, large ones read each operand less often: 32 experts of 4096 x 2048,
-  // forward, 16 rows each: 32 x 64 98 us, 256 x 256 128; 96 rows: 128 x 128 126, 256 x 256 133, 32 x 64 204; 256 rows: 252,
-  // 170 and 410.
+  // forward, 16 rows each: 32 x 64 83 us, 128 x 256 91, 256 x 256 94; 64 rows: 158, 99 and 102; 256 rows: 419, 193 and 182.
   struct Cost { int bm, bn; double step, rate; };  // microseconds, TB/s
-  static const Cost forward[] = {{32, 64, 0.22, 5.6}, {64, 256, 0.78, 3.0}, {128, 128, 0.69, 4.8}, {128, 256, 0.93, 3.5}, {256, 256, 1.31, 4.1}};
-  static const Cost grad_x[] = {{32, 64, 0.16, 4.3}, {64, 256, 0.68, 5.2}, {128, 128, 0.64, 4.0}, {128, 256, 1.02, 3.5}, {256, 256, 1.27, 5.0}};
+  static const Cost forward[] = {{32, 64, 0.20, 6.4}, {64, 256, 0.93, 4.2}, {128, 128, 0.64, 5.2}, {128, 256, 0.92, 6.2}, {256, 256, 1.15, 5.2}};
+  static const Cost grad_x[] = {{32, 64, 0.16, 4.8}, {64, 256, 0.83, 6.6}, {128, 128, 0.64, 5.1}, {128, 256, 1.15, 5.2}, {256, 256, 1.40, 5.2}};
   const Cost *const tiles = KIND == kForward ? forward : grad_x;
   const double used = (double)(g.rows < g.X ? g.rows : g.X), mean = (double)g.rows / used, bytes = used * g.N * g.K * sizeof(T);
   const bool cached = bytes <= (double)((int64_t)256 << 20);  // the card's last cache
@@ -345,7 +344,7 @@ int experts_panels(futhark_context *ctx, const char *who, hipStream_t stream, T 
     }
   }
   // weights that no cache can hold until the next call are read past it where nearly every block is read once: 32 blocks
-  // of 4096 x 2048, 110 -> 95 us; 8 of them, which it holds, 22 -> 31; 128 of 2048 x 768 where a few are read twice, 101 -> 146
+  // of 4096 x 2048, 94 -> 83 us; 8 of them, which it holds, 27 -> 33
   const bool once = 4 * mean <= 3 * tiles[best].bm && !cached;
   switch (best) {
     case 0:

@@ -10,7 +10,7 @@
 // through registers (buffer_load ... lds, 16 bytes a lane), some steps ahead of the products.  The buffer descriptor ends
 // at the expert's last row, so what a ragged tile would read beyond it is zero and costs no memory access.
 //
-// What bounds it: with few rows an expert the blocks' bytes (32 blocks of 4096 x 2048: 98 us, 5.5 TB/s), with many the
+// What bounds it: with few rows an expert the blocks' bytes (32 blocks of 4096 x 2048, 4 rows each: 77 us, 7.0 TB/s), with many the
 // matrix cores' clock under power: 2048 rows each, 1220 TFLOP/s forward and 1140 for the gradient by xs, where a large
 // library product reaches 1430 to 1520.
 //
@@ -79,6 +79,7 @@ struct Tile {
   const T *p;
   int64_t ld, rest, summed;
   int64_t width;        // how much of the result's index there is from the tile's first on
+  int steps, first, now;  // FAST, lying: how many steps there are, which is taken first (then in turn), steps moved on
   uint32_t off[FAST ? kLoads : 1];
   __amdgpu_buffer_rsrc_t bounds;
   Piece<T> held[2][FAST ? 1 : kLoads];  // not FAST: two steps on their way to LDS
@@ -103,7 +104,7 @@ struct Tile {
   static __device__ __forceinline__ int twist(int r) { return DEPTH == 128 ? r & 15 : DEPTH == 64 ? (r >> 1) & 7 : (4 - (r >> 2)) & 3; }
   static __device__ __forceinline__ int spread(int k) { return (k & 3) | (((k >> 3) & 1) << 2); }
 
-  __device__ __forceinline__ void init(const T *base, int64_t ld_, int64_t rest_, int64_t summed_, int64_t width_) {
+  __device__ __forceinline__ void init(const T *base, int64_t ld_, int64_t rest_, int64_t summed_, int64_t width_, int first_) {
     p = (const T *)same(reinterpret_cast<int64_t>(base)); ld = ld_; rest = same(rest_); summed = summed_; width = width_;
     if (FAST) {
 #pragma unroll
@@ -112,6 +113,9 @@ struct Tile {
         source(i, threadIdx.x, &r, &c);
         off[i] = (uint32_t)(((int64_t)r * ld + c) * (int64_t)sizeof(T));
       }
+      steps = (int)((summed + DEPTH - 1) / DEPTH);
+      first = steps > 0 ? first_ / DEPTH % steps : 0;
+      now = 0;
       bound();
     }
   }
@@ -121,12 +125,13 @@ struct Tile {
     bounds = __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, (int)(bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : bytes), 0x00020000);
   }
 
-  // FAST: steps are counted from here on `steps` further, so that their offsets stay small whatever the operand's size.
-  __device__ __forceinline__ void move(int steps) {
-    const int64_t by = steps * DEPTH * (STANDING ? ld : 1);
-    p += by;
-    rest -= by;
-    summed -= steps * DEPTH;
+  // FAST: steps are counted from here on `by` further.  Standing: the descriptor moves along, so that offsets stay small
+  // whatever the operand's size.
+  __device__ __forceinline__ void move(int by) {
+    now += by;
+    if (!STANDING) return;
+    p += by * DEPTH * ld;
+    rest -= by * DEPTH * ld;
     bound();
   }
 
@@ -135,9 +140,18 @@ struct Tile {
   __device__ __forceinline__ void start(T *lds, int step) {
     int row, col;
     source(0, threadIdx.x, &row, &col);  // the same columns in every load of a thread: NT / (DEPTH / 8) rows on, twist() repeats
-    // lying: columns beyond the summed index are the next row's, and are not read
-    const bool dead = !STANDING && col >= summed - step * DEPTH;
-    const int at = (int)(step * DEPTH * (STANDING ? ld : 1) * (int64_t)sizeof(T));
+    bool dead = false;
+    int at;
+    if (STANDING) {
+      at = (int)(step * DEPTH * ld * (int64_t)sizeof(T));
+    } else {  // columns beyond the summed index are the next row's, and are not read
+      int t = now + step;
+      const bool over = t >= steps;
+      t += first;
+      if (t >= steps) t -= steps;
+      dead = over || col >= (int)summed - t * DEPTH;
+      at = t * DEPTH * (int)sizeof(T);
+    }
     char *to = (char *)lds + wave_id() * (kWave * 16);
 #pragma unroll
     for (int i = 0; i < kLoads; i++)
@@ -255,21 +269,28 @@ __device__ __forceinline__ void arrived() {
 
 // The operands of a tile whose rows begin at m0 and columns at n0 of expert e's result, which ends with row m_end.
 template <int KIND, class T, class TA>
-__device__ __forceinline__ void operand_a(TA &ta, int e, int64_t m0, int64_t m_end, int64_t summed, const T *A, const int32_t *offsets, const ProductShape &g) {
+__device__ __forceinline__ void operand_a(TA &ta, int e, int64_t m0, int64_t m_end, int64_t summed, int first, const T *A, const int32_t *offsets, const ProductShape &g) {
   if (KIND == kGradW)
-    ta.init(A + clamped(offsets, e, g.rows) * g.ldA + m0, g.ldA, summed ? (summed - 1) * g.ldA + g.M - m0 : 0, summed, g.M - m0);
+    ta.init(A + clamped(offsets, e, g.rows) * g.ldA + m0, g.ldA, summed ? (summed - 1) * g.ldA + g.M - m0 : 0, summed, g.M - m0, 0);
   else
-    ta.init(A + m0 * g.ldA, g.ldA, (m_end - m0 - 1) * g.ldA + g.K, g.K, m_end - m0);
+    ta.init(A + m0 * g.ldA, g.ldA, (m_end - m0 - 1) * g.ldA + g.K, g.K, m_end - m0, first);
 }
 template <int KIND, class T, class TB>
-__device__ __forceinline__ void operand_b(TB &tb, int e, int64_t n0, int64_t summed, const T *B, const int32_t *offsets, const ProductShape &g) {
+__device__ __forceinline__ void operand_b(TB &tb, int e, int64_t n0, int64_t summed, int first, const T *B, const int32_t *offsets, const ProductShape &g) {
   if (KIND == kGradW)
-    tb.init(B + clamped(offsets, e, g.rows) * g.ldB + n0, g.ldB, summed ? (summed - 1) * g.ldB + g.N - n0 : 0, summed, g.N - n0);
+    tb.init(B + clamped(offsets, e, g.rows) * g.ldB + n0, g.ldB, summed ? (summed - 1) * g.ldB + g.N - n0 : 0, summed, g.N - n0, 0);
   else if (KIND == kForward)
-    tb.init(B + (int64_t)e * g.blockB + n0 * g.ldB, g.ldB, (g.N - n0 - 1) * g.ldB + g.K, g.K, g.N - n0);
+    tb.init(B + (int64_t)e * g.blockB + n0 * g.ldB, g.ldB, (g.N - n0 - 1) * g.ldB + g.K, g.K, g.N - n0, first);
   else
-    tb.init(B + (int64_t)e * g.blockB + n0, g.ldB, (g.K - 1) * g.ldB + g.N - n0, g.K, g.N - n0);
+    tb.init(B + (int64_t)e * g.blockB + n0, g.ldB, (g.K - 1) * g.ldB + g.N - n0, g.K, g.N - n0, 0);
 }
+// Where a tile's sums begin (they go round to what lies before).  Rows of W that are a power of two apart would all be read
+// at the same column at the same time, which meets in few of the memory's channels: so every die, and every expert on it,
+// begins elsewhere; the tiles that share rows in an L2 stay together.  32 blocks of 4096 x 2048, 16 rows each: 97 -> 83 us;
+// of 2048 x 4096, 94 -> 86; 96 rows each in tiles of 256 x 256: 133 -> 110; nothing where rows are 1.4 or 5 times a power of
+// two apart, or W is in a cache.  (A beginning for every column of tiles: 32 x 64 as much, 128 x 128 up to 10 % slower.)
+template <int KIND>
+__device__ __forceinline__ int first_column(int e) { return KIND == kForward ? ((int)blockIdx.x % kXcds + e) * 768 : 0; }
 // How long its sums are, and where its result goes.
 template <int KIND>
 __device__ __forceinline__ int64_t sum_length(int e, const int32_t *offsets, const ProductShape &g) {
@@ -411,8 +432,8 @@ __global__ __launch_bounds__(WM *WN *kWave) void experts_any_kernel(TO *__restri
   if (!place_product<KIND, BM, BN>(&e, &m0, &n0, &m_end, &half, offsets, g)) return;
   const int64_t summed = sum_length<KIND>(e, offsets, g);
   if (ADD && summed == 0) return;
-  operand_a<KIND>(ta, e, m0, m_end, summed, A, offsets, g);
-  operand_b<KIND>(tb, e, n0, summed, B, offsets, g);
+  operand_a<KIND>(ta, e, m0, m_end, summed, 0, A, offsets, g);
+  operand_b<KIND>(tb, e, n0, summed, 0, B, offsets, g);
   TO *const out = result_of<KIND>(C, e, g);
   const int wm = wave_id() / WN, wn = wave_id() % WN;
   Acc acc[NI][MI] = {};
@@ -487,8 +508,9 @@ __device__ __forceinline__ void multiply_small(int e, int64_t m0, int64_t n0, in
   TB tb;
   const int64_t summed = sum_length<KIND>(e, offsets, g);
   if (ADD && summed == 0) return;
-  operand_a<KIND>(ta, e, m0, m_end, summed, A, offsets, g);
-  operand_b<KIND>(tb, e, n0, summed, B, offsets, g);
+  const int first = first_column<KIND>(e);
+  operand_a<KIND>(ta, e, m0, m_end, summed, first, A, offsets, g);
+  operand_b<KIND>(tb, e, n0, summed, first, B, offsets, g);
   TO *const out = result_of<KIND>(C, e, g);
   const int wm = wave_id() / WN, wn = wave_id() % WN;
   Acc acc[NI][MI] = {};
@@ -582,9 +604,10 @@ __device__ __forceinline__ void multiply_large(const Parts<T> lds, int e, int64_
   TB col;
   const int64_t summed = sum_length<KIND>(e, offsets, g);
   if (ADD && summed == 0) return;
-  operand_a<KIND>(up, e, m0, m_end, summed, A, offsets, g);
-  operand_a<KIND>(low, e, m0 + HM, m_end, summed, A, offsets, g);
-  operand_b<KIND>(col, e, n0, summed, B, offsets, g);
+  const int first = first_column<KIND>(e);
+  operand_a<KIND>(up, e, m0, m_end, summed, first, A, offsets, g);
+  operand_a<KIND>(low, e, m0 + HM, m_end, summed, first, A, offsets, g);
+  operand_b<KIND>(col, e, n0, summed, first, B, offsets, g);
   TO *const out = result_of<KIND>(C, e, g);
   const int wm = wave_id() / WN, wn = wave_id() % WN;
   Acc acc[2][NI][MI] = {};
