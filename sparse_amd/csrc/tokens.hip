@@ -278,8 +278,8 @@ bool direct_to_lds(const T *p, int64_t ld, int64_t width) {
   return (uintptr_t)p % 16 == 0 && ld >= width && ld % 8 == 0 && ld <= ((int64_t)1 << 20);
 }
 
-// ANY: the kernel for any strides and alignment.
-template <class T, class TO, int KIND, int BM, int BN, int DEPTH, int WM, int WN, bool ADD, bool ONCE = false, bool ANY = false>
+enum { kSteps = 0, kAny = 1, kFew = 2 };  // the kernel: experts_kernel, experts_any_kernel, experts_few_kernel
+template <class T, class TO, int KIND, int BM, int BN, int DEPTH, int WM, int WN, bool ADD, bool ONCE = false, int KERNEL = kSteps>
 int launch_experts(futhark_context *ctx, const char *who, hipStream_t stream, TO *C, const T *A, const T *B, const int32_t *offsets,
                    ProductShape g) {
   const int64_t n_tiles = cdiv(g.N, BN);
@@ -301,7 +301,9 @@ int launch_experts(futhark_context *ctx, const char *who, hipStream_t stream, TO
   SAMD_TRY(check_blocks(ctx, who, blocks));
   g.m_tiles = (int)m_tiles;
   g.n_tiles = (int)n_tiles;
-  if constexpr (ANY)
+  if constexpr (KERNEL == kFew)
+    TOK_LAUNCH(ctx, (experts_few_kernel<T, TO, BM, BN, DEPTH, WM, WN, ADD>), blocks, WM * WN * kWave, stream, C, A, B, offsets, g);
+  else if constexpr (KERNEL == kAny)
     TOK_LAUNCH(ctx, (experts_any_kernel<T, TO, KIND, BM, BN, DEPTH, WM, WN, ADD>), blocks, WM * WN * kWave, stream, C, A, B, offsets, g);
   else
     TOK_LAUNCH(ctx, (experts_kernel<T, TO, KIND, BM, BN, DEPTH, WM, WN, ADD, ONCE>), blocks, WM * WN * kWave, stream, C, A, B, offsets, g);
@@ -313,8 +315,8 @@ int experts_panels(futhark_context *ctx, const char *who, hipStream_t stream, T 
                    const ProductShape &g) {
   const bool fast = direct_to_lds(A, g.ldA, g.K) && g.K % 8 == 0 && direct_to_lds(B, g.ldB, KIND == kForward ? g.K : g.N) && g.blockB % 8 == 0;
   if (!fast) {
-    if (g.rows <= 48 * g.X) return launch_experts<T, T, KIND, 32, 64, 128, 1, 4, false, false, true>(ctx, who, stream, C, A, B, offsets, g);
-    return launch_experts<T, T, KIND, 128, 128, 64, 2, 2, false, false, true>(ctx, who, stream, C, A, B, offsets, g);
+    if (g.rows <= 48 * g.X) return launch_experts<T, T, KIND, 32, 64, 128, 1, 4, false, false, kAny>(ctx, who, stream, C, A, B, offsets, g);
+    return launch_experts<T, T, KIND, 128, 128, 64, 2, 2, false, false, kAny>(ctx, who, stream, C, A, B, offsets, g);
   }
   // The tile whose launch is estimated to end first: rounds of the card's CUs, at the time that a tile takes for 64 of the
   // summed index, or one pass over the blocks where no cache holds them, at the rate that a tile's loads reach (64 bytes of
@@ -362,13 +364,23 @@ int experts_panels(futhark_context *ctx, const char *who, hipStream_t stream, T 
 template <class T, class TO, bool ADD>
 int experts_weights(futhark_context *ctx, const char *who, hipStream_t stream, TO *C, const T *A, const T *B, const int32_t *offsets,
                     const ProductShape &g) {
+  // small tiles where large ones would leave CUs without work (a tile's sum is one workgroup's): 8 blocks of 512 x 256, 1024
+  // rows each: 64 x 64 10 us, 128 x 128 14; 30 of 208 x 2024, 960 tiles of 128 x 128: 74 and 46
+  const bool small = g.X * cdiv(g.M, 128) * cdiv(g.N, 128) <= 128;
   if (!(direct_to_lds(A, g.ldA, g.M) && direct_to_lds(B, g.ldB, g.N))) {
-    if (g.rows <= 48 * g.X) return launch_experts<T, TO, kGradW, 64, 64, 32, 2, 2, ADD, false, true>(ctx, who, stream, C, A, B, offsets, g);
-    return launch_experts<T, TO, kGradW, 128, 128, 64, 2, 2, ADD, false, true>(ctx, who, stream, C, A, B, offsets, g);
+    if (small || g.rows <= 48 * g.X) return launch_experts<T, TO, kGradW, 64, 64, 32, 2, 2, ADD, false, kAny>(ctx, who, stream, C, A, B, offsets, g);
+    return launch_experts<T, TO, kGradW, 128, 128, 64, 2, 2, ADD, false, kAny>(ctx, who, stream, C, A, B, offsets, g);
   }
-  // as above: tiles enough for every CU to have a large one, and work in them: with few rows a tile is all writing, and two
-  // small ones on a CU overlap it better (16 rows an expert: 145 us against 150)
-  if (g.X * cdiv(g.M, 256) * cdiv(g.N, 256) >= 256 && g.rows > 64 * g.X) return launch_experts<T, TO, kGradW, 256, 256, 64, 2, 4, ADD>(ctx, who, stream, C, A, B, offsets, g);
+  if (g.rows <= 160 * g.X) {
+    // past the caches unless rows of dw share their lines: few sums leave the cache time to join the parts (110 blocks of
+    // 2888 x 688, 16 rows each: 149 us, past it 187; 192 rows: 279 and 215)
+    ProductShape few = g;
+    few.stream = g.stream && (((uintptr_t)C | g.ldC * sizeof(TO) | g.blockC * sizeof(TO)) % 128 == 0 || g.rows > 64 * g.X);
+    return launch_experts<T, TO, kGradW, 128, 128, 32, 2, 2, ADD, false, kFew>(ctx, who, stream, C, A, B, offsets, few);
+  }
+  if (small) return launch_experts<T, TO, kGradW, 64, 64, 32, 1, 4, ADD>(ctx, who, stream, C, A, B, offsets, g);
+  // as above: tiles enough for every CU to have a large one
+  if (g.X * cdiv(g.M, 256) * cdiv(g.N, 256) >= 256) return launch_experts<T, TO, kGradW, 256, 256, 64, 2, 4, ADD>(ctx, who, stream, C, A, B, offsets, g);
   return launch_experts<T, TO, kGradW, 128, 128, 32, 2, 2, ADD>(ctx, who, stream, C, A, B, offsets, g);
 }
 

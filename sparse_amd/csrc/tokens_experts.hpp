@@ -572,6 +572,63 @@ __device__ __forceinline__ void multiply_small(int e, int64_t m0, int64_t n0, in
   }
 }
 
+// dW of experts with few rows: nearly all of it is writing, so a workgroup keeps little (32 KiB of LDS, one slice of the rows
+// at a time) and four or five of them on a CU overlap.  32 blocks of 4096 x 2048, 16 rows each: 87 us, 6.2 TB/s, where four
+// stages and two workgroups take 142; 64 rows each: 117 and 150; 128 rows: 148 and 169; 256 rows: 218 and 218 (tiles of
+// 256 x 256).  Slices of 64: 16 rows 125; tiles of 64 x 256 90, of 64 x 128 96.
+template <class T, class TO, int BM, int BN, int DEPTH, int WM, int WN, bool ADD>
+__global__ __launch_bounds__(WM *WN *kWave) void experts_few_kernel(TO *__restrict__ C, const T *__restrict__ A, const T *__restrict__ B,
+                                                                    const int32_t *__restrict__ offsets, ProductShape g) {
+  constexpr int NT = WM * WN * kWave, KK = DEPTH / 32;
+  constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
+  using TA = Tile<T, BM, DEPTH, true, NT, true>;
+  using TB = Tile<T, BN, DEPTH, true, NT, true>;
+  using Acc = typename Mfma<T>::Acc;
+  using Frag = typename Mfma<T>::Frag;
+  constexpr bool rounded = std::is_same<T, TO>::value && !ADD;
+  __shared__ __align__(128) T lds[rounded ? BM * BN : (BM + BN) * DEPTH];
+  static_assert((BM + BN) * DEPTH <= BM * BN, "the slices fit where the result goes later");
+  T *const a = lds, *const b = lds + BM * DEPTH;
+  int e, half;
+  int64_t m0, n0, m_end;
+  if (!place_product<kGradW, BM, BN>(&e, &m0, &n0, &m_end, &half, offsets, g)) return;
+  const int64_t summed = sum_length<kGradW>(e, offsets, g);
+  if (ADD && summed == 0) return;
+  TA ta;
+  TB tb;
+  operand_a<kGradW>(ta, e, m0, m_end, summed, 0, A, offsets, g);
+  operand_b<kGradW>(tb, e, n0, summed, 0, B, offsets, g);
+  TO *const out = result_of<kGradW>(C, e, g);
+  const int wm = wave_id() / WN, wn = wave_id() % WN;
+  Acc acc[NI][MI] = {};
+  for (int64_t k0 = 0; k0 < summed; k0 += DEPTH) {
+    ta.start(a, 0);
+    tb.start(b, 0);
+    arrived<0>();
+    Frag fa[KK][MI], fb[KK][NI];
+#pragma unroll
+    for (int kk = 0; kk < KK; kk++) {
+#pragma unroll
+      for (int j = 0; j < NI; j++) fb[kk][j] = TB::fragment(b, wn * (BN / WN) + j * 16, kk);
+#pragma unroll
+      for (int i = 0; i < MI; i++) fa[kk][i] = TA::fragment(a, wm * (BM / WM) + i * 16, kk);
+    }
+    ta.move(1);
+    tb.move(1);
+    __syncthreads();  // everybody has read
+#pragma unroll
+    for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+      for (int j = 0; j < NI; j++)
+#pragma unroll
+        for (int i = 0; i < MI; i++) acc[j][i] = Mfma<T>::go(fb[kk][j], fa[kk][i], acc[j][i]);
+  }
+  if constexpr (rounded)
+    store_rounded<T, BM, BN, WM, WN>(lds + wave_id() * (BM / WM * (BN / WN)), out, acc, m0, n0, m_end, g);
+  else
+    store_product<T, TO, ADD, BM, BN, WM, WN>(out, acc, m0, n0, m_end, g);
+}
+
 // Eight waves, two on each SIMD, one workgroup on a CU.  LDS holds two steps of 64 of the summed index, so that a row gives
 // whole cache lines; each has three parts that are loaded and given up by themselves: the upper rows, the lower rows, and
 // all columns.  A step is two phases: read the columns' and the upper rows' fragments, multiply; read the lower rows'
