@@ -586,11 +586,19 @@ int sparse_amd_tokens_combine_grad(struct futhark_context *ctx, void *stream, in
                                           {"pos", pos, n, K, K, 4}, {"weights", weights, n, K, K, 4}}));
       if (n == 0 || K == 0) return 0;
       SAMD_TRY(check_blocks(ctx, who, n));
-      const auto go = [&](auto kernel) -> int {
-        TOK_LAUNCH(ctx, kernel, n, kThreads, (hipStream_t)stream, (T *)dys, lddys, dweights, (const T *)dy, lddy, (const T *)ys, ldys, D, (int)K, pos, slots, weights);
+      const auto go = [&](auto waves, auto at_once) -> int {
+        constexpr int W = decltype(waves)::value, J = decltype(at_once)::value;
+        const auto kernel = n * K * D * (int64_t)sizeof(T) > kStreamBytes ? combine_grad_kernel<T, W, J, true> : combine_grad_kernel<T, W, J, false>;
+        TOK_LAUNCH(ctx, kernel, W == 1 ? cdiv(n, kWaves) : n, kThreads, (hipStream_t)stream, (T *)dys, lddys, dweights, (const T *)dy, lddy, (const T *)ys, ldys, n, D, (int)K, pos, slots, weights);
         return 0;
       };
-      return n * K * D * (int64_t)sizeof(T) > kStreamBytes ? go(combine_grad_kernel<T, true>) : go(combine_grad_kernel<T, false>);
+      const auto choose = [&](auto waves) -> int {
+        return K <= 2 ? go(waves, std::integral_constant<int, 2>()) : K <= 4 ? go(waves, std::integral_constant<int, 4>()) : go(waves, std::integral_constant<int, 8>());
+      };
+      // choices that are not there cost their share of sums, registers and waiting: 8863 tokens of 1728 bf16, 1 place each, 8 at
+      // once 50 us, 2 at once 21.  A wave to itself where a row is two rounds of it at most: 16384 tokens of 256, 4 places each,
+      // a workgroup 106 us, a wave 31; of 2048, 8 places each, 212 and 293.
+      return cdiv(D, kPer<T>) <= 2 * kWave ? choose(std::integral_constant<int, 1>()) : choose(std::integral_constant<int, kWaves>());
     });
   });
 }

@@ -140,16 +140,18 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(T *__restrict__ y, in
   }
 }
 
-// One workgroup per token, its waves side by side along the row; eight choices at once share one reading of dy.  The dot
-// products are summed lane, wave, workgroup: the same order every time.
-template <class T, bool STREAM>
+// W waves per token, side by side along its row; J choices at once share one reading of dy.  The dot products are summed
+// lane, wave, token: the same order every time.
+template <class T, int W, int J, bool STREAM>
 __global__ __launch_bounds__(kThreads) void combine_grad_kernel(T *__restrict__ dys, int64_t lddys, float *__restrict__ dw,
                                                                 const T *__restrict__ dy, int64_t lddy, const T *__restrict__ ys,
-                                                                int64_t ldys, int64_t D, int K, const int32_t *__restrict__ pos,
+                                                                int64_t ldys, int64_t n, int64_t D, int K, const int32_t *__restrict__ pos,
                                                                 int64_t slots, const float *__restrict__ w) {
-  constexpr int J = 8;
+  static_assert(W == 1 || W == kWaves, "a token has a wave or a workgroup");
   __shared__ float part[kWaves][J];
-  const int64_t t = blockIdx.x;
+  const int64_t t = W == 1 ? (int64_t)blockIdx.x * kWaves + wave_id() : blockIdx.x;
+  if (t >= n) return;
+  const int first = W == 1 ? lane_id() : (int)threadIdx.x;
   for (int j0 = 0; j0 < K; j0 += J) {
     int64_t at[J];
     float f[J], dot[J];
@@ -161,7 +163,7 @@ __global__ __launch_bounds__(kThreads) void combine_grad_kernel(T *__restrict__ 
       f[j] = in ? w[t * K + j0 + j] : 0.0f;
       dot[j] = 0.0f;
     }
-    for (int64_t c = (int64_t)threadIdx.x * kPer<T>; c < D; c += kThreads * kPer<T>) {
+    for (int64_t c = (int64_t)first * kPer<T>; c < D; c += W * kWave * kPer<T>) {
       const Piece<T> g = load_piece<true>(dy + t * lddy + c, D - c);
       Piece<T> p[J];
 #pragma unroll
@@ -182,8 +184,13 @@ __global__ __launch_bounds__(kThreads) void combine_grad_kernel(T *__restrict__ 
 #pragma unroll
     for (int j = 0; j < J; j++) {
       const float s = wave_sum(dot[j]);
-      if (lane_id() == 0) part[wave_id()][j] = s;
+      if (W == 1) {
+        if (lane_id() == 0 && j0 + j < K) dw[t * K + j0 + j] = s;
+      } else if (lane_id() == 0) {
+        part[wave_id()][j] = s;
+      }
     }
+    if (W == 1) continue;
     __syncthreads();
     if (threadIdx.x < J && j0 + (int)threadIdx.x < K) {
       float s = 0.0f;
