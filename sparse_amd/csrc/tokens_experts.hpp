@@ -377,8 +377,8 @@ __device__ __forceinline__ void store_product(TO *out, const Acc (&acc)[NI][MI],
 }
 
 // Rounded to 16 bits: through `mine`, LDS that only this wave uses, so that a row leaves the wave in pieces of 16 bytes that
-// lie side by side (a wave's 64 columns are a cache line; written four columns a lane, 32 blocks of 4096 x 2048 for few rows took
-// 214 us where this takes 150).  The pieces of a row are permuted by the row's number: the lanes that write the same
+// lie side by side (a wave's 64 columns are a cache line; written four columns a lane, dW of 32 blocks of 4096 x 2048 for few
+// rows, in four stages, took 214 us where this took 150).  The pieces of a row are permuted by the row's number: the lanes that write the same
 // columns of 16 rows would all meet in a few banks.
 template <class T, int BM, int BN, int WM, int WN, class Acc, int NI, int MI>
 __device__ __forceinline__ void store_rounded(T *mine, T *out, const Acc (&acc)[NI][MI], int64_t m0, int64_t n0, int64_t m_end, const ProductShape &g) {

@@ -339,6 +339,25 @@ def test_experts_and_their_gradients(tk, t, counts, dropped, D, F, lay):
         at += k
 
 
+# many experts, so that the card has more than one round of tiles: a last round of half tiles, sums that begin at another column
+# for every expert, results written past the caches
+@pytest.mark.parametrize("counts,D,F", [([400, 389, 511, 257] * 5, 2056, 2048), ([20, 100, 130, 64] * 15, 1528, 328), ([3, 0, 1] * 17, 2048, 1032), ([170, 1, 350] * 12, 1032, 2064)])
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+def test_rounds_of_tiles(tk, t, counts, D, F):
+    g = gen(D + F + len(counts))
+    X, n = len(counts), sum(counts)
+    r = routed(tk(t), g, counts, 0)
+    xs, dys, W = normal(g, (n, D), DT[t]), normal(g, (n, F), DT[t]), normal(g, (X, F, D), DT[t])
+    ys, dxs, dW = tk(t).experts(xs, W, r), tk(t).experts_grad_x(dys, W, r), tk(t).experts_grad_w(dys, xs, r)
+    at = 0
+    for e, k in enumerate(counts):
+        a, b, w = xs[at:at + k].double(), dys[at:at + k].double(), W[e].double()
+        close(ys[at:at + k], a @ w.t(), a.abs() @ w.abs().t(), D)
+        close(dxs[at:at + k], b @ w, b.abs() @ w.abs(), F)
+        close(dW[e], b.t() @ a, b.abs().t() @ a.abs(), k)
+        at += k
+
+
 def test_an_experts_nan_stays_with_it(tk):
     g = gen(3)
     counts = [40, 50, 70]
