@@ -26,7 +26,8 @@ struct Piece {
   T v[kPer<T>];
 };
 
-typedef uint32_t __attribute__((ext_vector_type(4), aligned(2))) Quad;  // 16 bytes at any element's address
+typedef uint32_t __attribute__((ext_vector_type(4), aligned(2), may_alias)) Quad;  // 16 bytes at any element's address
+// (a copy of bytes instead is stored in parts where the compiler joins it with the elements of a tail)
 
 // The `left` elements (kPer or fewer) of a piece at p; what is not there reads as zero.  ONCE: nobody will read them again
 // soon, so they are not kept in the caches in the place of what will be (a non-temporal load).
@@ -51,13 +52,10 @@ __device__ __forceinline__ Piece<T> load_piece(const T *p, int64_t left) {
 template <bool STREAM = false, class T>
 __device__ __forceinline__ void store_piece(T *p, const Piece<T> &r, int64_t left) {
   if (left >= kPer<T>) {
-    if (STREAM) {
-      Quad q;
-      __builtin_memcpy(&q, &r, 16);
-      __builtin_nontemporal_store(q, (Quad *)p);
-    } else {
-      __builtin_memcpy(p, &r, 16);
-    }
+    Quad q;
+    __builtin_memcpy(&q, &r, 16);
+    if (STREAM) __builtin_nontemporal_store(q, (Quad *)p);
+    else *(Quad *)p = q;
   } else if (left > 0) {
 #pragma unroll
     for (int i = 0; i < kPer<T> - 1; i++)
@@ -65,9 +63,9 @@ __device__ __forceinline__ void store_piece(T *p, const Piece<T> &r, int64_t lef
   }
 }
 
-// A result larger than the L2s of the card (8 x 4 MiB) is written past them: its lines would push out each other and what
-// is being read (non-temporal stores; 16384 rows of 8 KiB looked up: 45 -> 32 us, a gradient of 512 MiB: 157 -> 88 us).
-// A smaller one is left to the caches, where the next kernel finds it.
+// A result larger than the L2s of the card (8 x 4 MiB) is written past them (non-temporal stores): its lines would push out
+// what is being read.  A smaller one is left to the caches, where the next kernel finds it.  16384 rows of 8 KiB looked up:
+// 43 -> 40 us; 32 blocks of dW, 512 MiB: 127 -> 101 us.
 constexpr int64_t kStreamBytes = (int64_t)32 << 20;
 
 // kPer<T> sums held in 32 bits, rounded once to TO (16 or 32 bits) and stored; ADD: added to what is there first.

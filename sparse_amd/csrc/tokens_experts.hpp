@@ -247,12 +247,15 @@ struct TileCounts {
 
 template <class T, class TO, bool ADD>
 __device__ __forceinline__ void store_four(TO *p, const typename Mfma<T>::Acc &a, int64_t left) {
+  typedef uint32_t __attribute__((ext_vector_type(sizeof(TO)), aligned(2), may_alias)) Four;
   if (left >= 4) {
     TO o[4];
     if (ADD) __builtin_memcpy(o, p, sizeof o);
 #pragma unroll
     for (int i = 0; i < 4; i++) o[i] = (TO)(ADD ? (float)o[i] + a[i] : a[i]);
-    __builtin_memcpy(p, o, sizeof o);
+    Four q;
+    __builtin_memcpy(&q, o, sizeof o);
+    *(Four *)p = q;
   } else {
 #pragma unroll
     for (int i = 0; i < 4; i++)

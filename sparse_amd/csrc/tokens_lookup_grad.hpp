@@ -23,7 +23,9 @@ struct GradShape {
   int chunk;         // positions in a chunk: a multiple of 8
 };
 
-constexpr int kFillPieces = 4;
+// Zeros are fastest from many short waves in the order of memory: 2 pieces of a row a lane; 16384 rows into 131072 of 2048 bf16
+// 107 us, 4 pieces 117, 1 piece 150.
+constexpr int kFillPieces = 2;
 
 // Sum of a chunk's part of a run, as two rows of 32-bit sums per chunk: [chunk][head, tail][segs * 64 * kPer].
 template <class T>
