@@ -304,22 +304,7 @@ __device__ __forceinline__ int64_t sum_length(int e, const int32_t *offsets, con
 template <int KIND, class TO>
 __device__ __forceinline__ TO *result_of(TO *C, int e, const ProductShape &g) { return KIND == kGradW ? C + (int64_t)e * g.blockC : C; }
 
-// The expert with the `at`-th most rows of X, 64 at most.
-__device__ __forceinline__ int by_rows(const int32_t *offsets, int at, int X, int64_t rows) {
-  const int l = lane_id();
-  const int mine = l < X ? (int)(clamped(offsets, l + 1, rows) - clamped(offsets, l, rows)) : 0;
-  int before = 0;
-  for (int e = 0; e < X; e++) {
-    const int its = __builtin_amdgcn_readlane(mine, e);
-    before += its > mine || (its == mine && e < l);
-  }
-  return __builtin_ctzll(__ballot(l < X && before == at));
-}
-
 // Where the workgroup's tile is.  False: it has none.
-//
-// Tiles of dW cost what their expert has rows: large ones are begun in the order of the rows, so that the last to end are short
-// (16 experts of 334 to 2223 rows, 4096 x 2048: 271 us, in the order of the experts 282).
 //
 // A last round of a few tiles of 256 x 256 would leave most CUs idle for as long as any other: if it fills half of them or
 // fewer (g.split: the launch has workgroups enough) each of its tiles is cut into its upper and its lower rows; *half =
@@ -336,7 +321,6 @@ __device__ __forceinline__ bool place_product(int *e, int64_t *m0, int64_t *n0, 
     const int per = (g.m_tiles * g.n_tiles + kXcds - 1) / kXcds * kXcds;
     *e = id / per;
     const int t = place_of(id - *e * per, g.m_tiles * g.n_tiles);
-    if (BM == 256 && g.X <= kWave && t >= 0) *e = by_rows(offsets, *e, g.X, g.rows);
     if (t < 0) return false;
     tile_at(t, g.m_tiles, g.n_tiles, &m, &n);
     *m0 = (int64_t)m * BM;
