@@ -576,11 +576,11 @@ __device__ __forceinline__ void multiply_small(int e, int64_t m0, int64_t n0, in
 }
 
 // dW of experts with few rows: nearly all of it is writing, so a workgroup keeps little (32 KiB of LDS, one slice of the rows
-// at a time) and four or five of them on a CU overlap.  32 blocks of 4096 x 2048, 16 rows each: 87 us, 6.2 TB/s, where four
-// stages and two workgroups take 142; 64 rows each: 117 and 150; 128 rows: 148 and 169; 256 rows: 218 and 218 (tiles of
-// 256 x 256).  Slices of 64: 16 rows 125; tiles of 64 x 256 90, of 64 x 128 96.
+// at a time; 128 registers) and four of them on a CU overlap.  32 blocks of 4096 x 2048, 16 rows each: 90 us, 6.0 TB/s, where
+// three workgroups take 102, and four stages and two workgroups 142; 128 rows: 136, 157 and 169; 256 rows: as long as tiles of
+// 256 x 256.  Slices of 64: 16 rows 125; tiles of 64 x 256 and 64 x 128 3 and 10 % more.
 template <class T, class TO, int BM, int BN, int DEPTH, int WM, int WN, bool ADD>
-__global__ __launch_bounds__(WM *WN *kWave) void experts_few_kernel(TO *__restrict__ C, const T *__restrict__ A, const T *__restrict__ B,
+__global__ __launch_bounds__(WM *WN *kWave, 4) void experts_few_kernel(TO *__restrict__ C, const T *__restrict__ A, const T *__restrict__ B,
                                                                     const int32_t *__restrict__ offsets, ProductShape g) {
   constexpr int NT = WM * WN * kWave, KK = DEPTH / 32;
   constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
