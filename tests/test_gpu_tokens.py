@@ -219,6 +219,22 @@ def route_ref(c, X):
     src[:live] = order[:live]
     return pos.reshape(c.shape), src, np.searchsorted(key[order], np.arange(X + 1))
 
+# nearly all of the result is zeros, whole and with rows apart
+@pytest.mark.parametrize("V,D,pad", [(70001, 2048, 0), (40003, 1801, 7)])
+def test_few_ids_of_a_large_table(tk, V, D, pad):
+    g = gen(V)
+    ids = torch.tensor([V - 1, 0, -1, 5, V, 5, V // 2], device="cuda")
+    dy = torch.randn((len(ids), D), generator=g, device="cuda")
+    base = torch.full((V, D + pad), 7.0, device="cuda")
+    out = base[:, :D]
+    assert tk("f32").lookup_grad(dy, ids, V, out=out) is out
+    want = {V - 1: dy[0], 0: dy[1], 5: dy[3] + dy[5], V // 2: dy[6]}
+    for v, row in want.items():
+        assert torch.equal(out[v], row)
+    out[list(want)] = 0.0
+    assert not out.any() and (base[:, D:] == 7.0).all()
+
+
 
 ROUTES = [(0, 2, 4), (1, 1, 1), (1, 8, 64), (64, 4, 1024), (65, 4, 3), (256, 4, 256), (1000, 8, 17), (1025, 8, 1000), (4096, 2, 8), (4097, 2, 8), (8192, 2, 64), (8193, 2, 1000), (5461, 3, 1024),
           (30001, 3, 128), (150000, 4, 1024), (600000, 2, 5)]
