@@ -8,7 +8,8 @@
 // One workgroup computes a BM x BN tile of one expert's result; sums are in 32 bits (v_mfma_f32_16x16x32) and rounded
 // once.  A step takes 32, 64 or 128 of the summed index: each operand's slice of it goes from memory to LDS without passing
 // through registers (buffer_load ... lds, 16 bytes a lane), some steps ahead of the products.  The buffer descriptor ends
-// at the expert's last row, so what a ragged tile would read beyond it is zero and costs no memory access.
+// with the expert's last row (its last chunk of 16 bytes), so what a ragged tile would read beyond it is zero and costs no
+// memory access.
 //
 // What bounds it: with few rows an expert the blocks' bytes (32 blocks of 4096 x 2048, 4 rows each: 77 us, 7.0 TB/s), with many the
 // matrix cores' clock under power: 2048 rows each, 1220 TFLOP/s forward and 1140 for the gradient by xs, where a large
@@ -77,7 +78,7 @@ struct Tile {
   static_assert(kLoads >= 1 && R * DEPTH * (int)sizeof(T) / 16 % NT == 0, "a tile is a whole number of loads for every thread");
 
   const T *p;
-  int64_t ld, rest, summed;
+  int64_t ld, rest, summed;  // FAST: rest in whole chunks
   int64_t width;        // how much of the result's index there is from the tile's first on
   int steps, first, now;  // FAST, lying: how many steps there are, which is taken first (then in turn), steps moved on
   uint32_t off[FAST ? kLoads : 1];
@@ -107,6 +108,10 @@ struct Tile {
   __device__ __forceinline__ void init(const T *base, int64_t ld_, int64_t rest_, int64_t summed_, int64_t width_, int first_) {
     p = (const T *)same(reinterpret_cast<int64_t>(base)); ld = ld_; rest = same(rest_); summed = summed_; width = width_;
     if (FAST) {
+      // The descriptor ends with a whole chunk: of one that it ended in, the four bytes that hold its end would read as zero, and
+      // a width that is odd would lose its last element.  Chunks begin on 16 bytes, so none reaches into memory that is not
+      // there, and what lies behind the width is of columns that are not written.
+      rest = (rest + 7) & ~(int64_t)7;
 #pragma unroll
       for (int i = 0; i < kLoads; i++) {
         int r, c;

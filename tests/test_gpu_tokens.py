@@ -354,6 +354,34 @@ def test_experts_and_their_gradients(tk, t, counts, dropped, D, F, lay):
             assert not dW[e].any() and torch.equal(added[e], start[e])
         at += k
 
+# ------------------------------------------------------------------------------------------------ experts in padded rows
+def padded(a, fill=NAN):
+    """The same values in rows (of blocks, one more row apart) that begin on 16 bytes, the next multiple of 8 elements long."""
+    base = torch.full((*a.shape[:-2], a.shape[-2] + (a.dim() == 3), (a.shape[-1] + 7) // 8 * 8), fill, dtype=a.dtype, device="cuda")
+    v = base[..., :a.shape[-2], :a.shape[-1]]
+    v.copy_(a)
+    return base, v
+
+
+# The last rows of an operand end inside a piece of 16 bytes, and inside one of 4: nothing of them may be lost.  The experts'
+# rows fill the last step of the sums exactly, by one row more and by one less; few and many of them (all tiles of the gradients).
+@pytest.mark.parametrize("counts,D,F", [([128, 64, 1, 0, 32], 65, 77), ([127, 129], 68, 257), ([64, 33], 257, 68), ([512, 1024], 130, 77), ([700, 511, 0, 641], 516, 259),
+                                        ([300, 1000], 1030, 2049), ([192], 4093, 4090), ([40, 24] * 8, 1027, 515), ([1, 2, 0, 3], 2051, 1025), ([1024, 2048, 1500], 1036, 2044)])
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+def test_experts_of_any_width_in_padded_rows(tk, t, counts, D, F):
+    g = gen(D + F)
+    X, n = len(counts), sum(counts)
+    r = routed(tk(t), g, counts, 0)
+    xs, dys, W = (padded(normal(g, shape, DT[t]))[1] for shape in ((n, D), (n, F), (X, F, D)))
+    ys, dxs, dW = tk(t).experts(xs, W, r), tk(t).experts_grad_x(dys, W, r), tk(t).experts_grad_w(dys, xs, r)
+    at = 0
+    for e, k in enumerate(counts):
+        a, b, w = xs[at:at + k].double(), dys[at:at + k].double(), W[e].double()
+        close(ys[at:at + k], a @ w.t(), a.abs() @ w.abs().t(), D)
+        close(dxs[at:at + k], b @ w, b.abs() @ w.abs(), F)
+        close(dW[e], b.t() @ a, b.abs().t() @ a.abs(), k)
+        at += k
+
 
 # many experts, so that the card has more than one round of tiles: a last round of half tiles, sums that begin at another column
 # for every expert, results written past the caches
