@@ -363,6 +363,13 @@ def padded(a, fill=NAN):
     return base, v
 
 
+def untouched(base, v, fill):
+    """What lies between the rows and blocks of v, a view of base, is `fill` still."""
+    around = torch.ones(base.shape, dtype=torch.bool, device="cuda")
+    around[..., :v.shape[-2], :v.shape[-1]] = False
+    return bool((base[around] == fill).all())
+
+
 # The last rows of an operand end inside a piece of 16 bytes, and inside one of 4: nothing of them may be lost.  The experts'
 # rows fill the last step of the sums exactly, by one row more and by one less; few and many of them (all tiles of the gradients).
 @pytest.mark.parametrize("counts,D,F", [([128, 64, 1, 0, 32], 65, 77), ([127, 129], 68, 257), ([64, 33], 257, 68), ([512, 1024], 130, 77), ([700, 511, 0, 641], 516, 259),
@@ -381,6 +388,32 @@ def test_experts_of_any_width_in_padded_rows(tk, t, counts, D, F):
         close(dxs[at:at + k], b @ w, b.abs() @ w.abs(), F)
         close(dW[e], b.t() @ a, b.abs().t() @ a.abs(), k)
         at += k
+
+
+# Every kernel of the gradient by W, into every kind of result.
+@pytest.mark.parametrize("counts,D,F", [([20, 0, 7], 72, 136), ([200, 0, 300], 72, 136), ([200, 0, 300, 180], 1040, 1288), ([400, 0, 170], 4096, 2048), ([40, 0, 30], 65, 77),
+                                        ([700, 0, 600], 65, 77), ([300, 0, 170], 2051, 1025), ([25, 3, 0, 9], 517, 1026)])
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("lay", ["rows", "padded"])
+def test_weight_gradients_into_and_onto_every_result(tk, t, counts, D, F, lay):
+    g = gen(D + F)
+    X, n = len(counts), sum(counts)
+    r = routed(tk(t), g, counts, 0)
+    xs, dys = normal(g, (n, D), DT[t]), normal(g, (n, F), DT[t])
+    if lay == "padded":
+        xs, dys = padded(xs)[1], padded(dys)[1]
+    for dtype, add in itertools.product((DT[t], torch.float32), (False, True)):
+        start = normal(g, (X, F, D), dtype)
+        base, out = padded(start, 3.0) if lay == "padded" else (None, start.clone())
+        assert tk(t).experts_grad_w(dys, xs, r, out=out, accumulate=add) is out
+        assert base is None or untouched(base, out, 3.0)
+        at = 0
+        for e, k in enumerate(counts):
+            a, b, s = xs[at:at + k].double(), dys[at:at + k].double(), start[e].double() * add
+            close(out[e], b.t() @ a + s, b.abs().t() @ a.abs() + s.abs(), k + add)
+            if k == 0:
+                assert torch.equal(out[e], start[e] if add else torch.zeros_like(start[e]))
+            at += k
 
 
 # many experts, so that the card has more than one round of tiles: a last round of half tiles, sums that begin at another column
