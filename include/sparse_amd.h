@@ -613,8 +613,8 @@ int sparse_amd_dcsr_f64_smvm(struct sparse_amd_group *g, struct sparse_amd_dvec_
  *     elements'.  The rows of a result lie apart (ld >= width); rows that are only read may have any stride, zero included;
  *   - every call names the HIP stream it runs on (NULL: the null stream) and touches neither the context's stream nor its
  *     memory: it allocates nothing, never waits, keeps nothing between calls, and may be captured into a graph.  What needs
- *     a workspace takes it as an argument (256-byte aligned, at least ..._workspace bytes, free for other use when the
- *     stream has passed the call; contents do not matter).  The calling thread's current device is left as it was;
+ *     a workspace takes it as an argument (256-byte aligned, at least ..._workspace bytes that no other argument shares,
+ *     free for other use when the stream has passed the call; contents do not matter).  The calling thread's current device is left as it was;
  *   - `type` is the element type of the panels: SPARSE_AMD_F32, SPARSE_AMD_F16, SPARSE_AMD_BF16 (experts...: the 16-bit ones).
  *     Sums are held in 32 bits and rounded once; values, weights and their gradients are 32-bit floats;
  *   - indices that come in have `id_bits` = 32 or 64 bits.  An id outside 0 .. V-1, or an expert outside 0 .. X-1, selects

@@ -478,6 +478,9 @@ int sparse_amd_tokens_lookup_grad(struct futhark_context *ctx, void *stream, int
           return sum_few_as<T, float, I>(ctx, s, accumulate != 0, (float *)dtable, (const T *)dy, (const I *)ids, vals, scale, p.g);
         }
         SAMD_TRY(check_work(ctx, who, work, work_bytes, p.bytes));
+        // it is written before the last of what is read has been
+        SAMD_TRY(check_panels(ctx, who, 1, {{"the workspace", work, 1, p.bytes, p.bytes, 1}, {"dy", dy, n, D, ldy, (int64_t)sizeof(T)},
+                                            {"ids", ids, 1, n, n, (int64_t)sizeof(I)}, {"vals", vals, 1, vals ? n : 0, n, 4}}));
         SAMD_TRY(order_ids<I>(ctx, s, (const I *)ids, p, !accumulate));
         if (out_type == type) return sum_ids_as<T, T>(ctx, s, accumulate != 0, (T *)dtable, (const T *)dy, vals, scale, p);
         return sum_ids_as<T, float>(ctx, s, accumulate != 0, (float *)dtable, (const T *)dy, vals, scale, p);
@@ -510,7 +513,9 @@ int sparse_amd_tokens_route(struct futhark_context *ctx, void *stream, const voi
       else if (n <= kOneGroupChoices)
         TOK_LAUNCH(ctx, (route_small_kernel<I, 16, 4>), 1, 1024, s, (const I *)chosen, (int)n, (int)X, bits, pos, src, offsets);
       else {
-        SAMD_TRY(check_work(ctx, who, work, work_bytes, sparse_amd_tokens_route_workspace(n, X)));
+        const int64_t need = sparse_amd_tokens_route_workspace(n, X);
+        SAMD_TRY(check_work(ctx, who, work, work_bytes, need));
+        SAMD_TRY(check_panels(ctx, who, 1, {{"the workspace", work, 1, need, need, 1}, {"chosen", chosen, 1, n, n, (int64_t)sizeof(I)}}));
         const Split sp(n);
         const Digits<0, I> d = {(const I *)chosen, nullptr, n, X, 0, 0};
         const bool self = n <= kSelfChoices;

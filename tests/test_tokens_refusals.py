@@ -99,6 +99,17 @@ def test_combine_grad_and_grad_x_refuse_overlaps(call):
     assert rc != 0 and "overlaps" in text
 
 
+# the workspace is written while the inputs are still read; where none is needed, what is given for one is not touched
+@pytest.mark.parametrize("f,change,words", [(grad, dict(n=300, work=B), "workspace overlaps dy"), (grad, dict(n=300, dy=W - 300 * 128 + 128, work=W), "workspace overlaps dy"),
+                                            (grad, dict(n=300, work=C), "workspace overlaps ids"), (grad, dict(n=300, vals=D + 512, work=D), "workspace overlaps vals"),
+                                            (route, dict(n=10000, work=A), "workspace overlaps chosen"), (route, dict(n=10000, work=A + 65536), "workspace overlaps chosen"),
+                                            (grad, dict(n=256, work=B), "no usable HIP device"), (route, dict(n=8192, work=A), "no usable HIP device"),
+                                            (grad, dict(n=300, dy=W - 300 * 128, work=W), "no usable HIP device")])
+def test_a_workspace_shares_nothing_with_what_is_read(call, f, change, words):
+    rc, text = f(call, **change)
+    assert rc != 0 and words in text, text
+
+
 @pytest.mark.parametrize("f,change", [(lookup, dict(n=0)), (lookup, dict(D=0)), (combine, dict(n=0)), (experts, dict(rows=0)), (experts, dict(F=0)),
                                       (grad, dict(n=0, acc=1)), (grad, dict(V=0)), (grad_w, dict(F=0))])
 def test_nothing_to_do_is_no_success_without_a_device(call, f, change):
