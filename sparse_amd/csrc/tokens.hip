@@ -114,10 +114,15 @@ int check_blocks(futhark_context *ctx, const char *who, int64_t blocks) {
   return 0;
 }
 
+// As many for a kernel that takes its workgroups' numbers from the grid's first dimension alone.
+int check_row(futhark_context *ctx, const char *who, int64_t blocks, int threads) {
+  return check_blocks(ctx, who, blocks * threads < (int64_t)1 << 32 ? blocks : (int64_t)1 << 32);
+}
+
 #define TOK_LAUNCH(ctx, kernel, blocks, threads, stream, ...)                                                  \
   do {                                                                                                         \
     SAMD_TRY(need_device(ctx));                                                                                \
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks)), dim3((unsigned)(threads)), 0, stream, __VA_ARGS__);    \
+    hipLaunchKernelGGL(kernel, grid_of(blocks, threads), dim3((unsigned)(threads)), 0, stream, __VA_ARGS__);        \
     SAMD_LAUNCH_CHECK(ctx);                                                                                    \
   } while (0)
 
@@ -182,6 +187,11 @@ struct GradPlan {
     part = c.take<float>(g.chunks > 1 ? g.chunks * 2 * g.segs * kWave * per : 0);
     bytes = c.used;
   }
+
+  // Workgroups of the launch that sums and zeroes (zeroes nothing until it has been told how), and of the one that joins.
+  void zero(int out_type) { g.fill = deal_rows(g.V, cdiv(g.D, 16 / type_size(out_type)), kFillPieces); }
+  int64_t sum_blocks() const { return cdiv(join_blocks() + g.fill.waves, kWaves); }
+  int64_t join_blocks() const { return g.chunks * g.segs; }
 };
 
 int check_work(futhark_context *ctx, const char *who, const void *work, int64_t have, int64_t need) {
@@ -230,15 +240,11 @@ int order_ids(futhark_context *ctx, hipStream_t stream, const I *ids, const Grad
 }
 
 template <class T, class TO, bool ADD, bool STREAM>
-int sum_ids(futhark_context *ctx, hipStream_t stream, TO *dE, const T *dy, const float *vals, float scale, GradPlan &p) {
-  if (!ADD) p.g.fill = deal_rows(p.g.V, cdiv(p.g.D, kPer<TO>), kFillPieces);
-  const int64_t blocks = cdiv(p.g.chunks * p.g.segs + p.g.fill.waves, kWaves);
-  SAMD_TRY(check_blocks(ctx, "lookup_grad", blocks));
-  SAMD_TRY(check_blocks(ctx, "lookup_grad", p.g.chunks * p.g.segs));
-  TOK_LAUNCH(ctx, (lookup_grad_kernel<T, TO, ADD, STREAM>), blocks, kThreads, stream, dE, dy, vals, scale, (const uint32_t *)p.keys,
+int sum_ids(futhark_context *ctx, hipStream_t stream, TO *dE, const T *dy, const float *vals, float scale, const GradPlan &p) {
+  TOK_LAUNCH(ctx, (lookup_grad_kernel<T, TO, ADD, STREAM>), p.sum_blocks(), kThreads, stream, dE, dy, vals, scale, (const uint32_t *)p.keys,
              (const int32_t *)p.items, (const uint8_t *)p.named, p.part, p.g);
   if (p.g.chunks > 1)
-    TOK_LAUNCH(ctx, (lookup_grad_join_kernel<T, TO, ADD, STREAM>), p.g.chunks * p.g.segs, kThreads, stream, dE, (const uint32_t *)p.keys, p.part, p.g);
+    TOK_LAUNCH(ctx, (lookup_grad_join_kernel<T, TO, ADD, STREAM>), p.join_blocks(), kThreads, stream, dE, (const uint32_t *)p.keys, p.part, p.g);
   return 0;
 }
 
@@ -251,7 +257,7 @@ int sum_few(futhark_context *ctx, hipStream_t stream, TO *dE, const T *dy, const
   const int64_t rows = (share < 16 * 1024 ? 16 * 1024 : share > 128 * 1024 ? 128 * 1024 : share) / (units * 16);
   const int fill_rows = (int)(rows < 1 ? 1 : rows > kFewFillRows ? kFewFillRows : rows);
   const int64_t blocks = g.segs + (ADD ? 0 : cdiv(g.V, fill_rows));
-  SAMD_TRY(check_blocks(ctx, "lookup_grad", blocks));
+  SAMD_TRY(check_row(ctx, "lookup_grad", blocks, kFewWaves * kWave));
   TOK_LAUNCH(ctx, (lookup_grad_few_kernel<T, TO, I, ADD, STREAM>), blocks, kFewWaves * kWave, stream, dE, dy, ids, vals, scale, g, fill_rows);
   return 0;
 }
@@ -265,7 +271,7 @@ int sum_few_as(futhark_context *ctx, hipStream_t stream, bool add, TO *dE, const
 
 // The gradient's table: written past the caches when all of it is written and it is large.
 template <class T, class TO>
-int sum_ids_as(futhark_context *ctx, hipStream_t stream, bool add, TO *dE, const T *dy, const float *vals, float scale, GradPlan &p) {
+int sum_ids_as(futhark_context *ctx, hipStream_t stream, bool add, TO *dE, const T *dy, const float *vals, float scale, const GradPlan &p) {
   if (add) return sum_ids<T, TO, true, false>(ctx, stream, dE, dy, vals, scale, p);
   if (p.g.V * p.g.D * (int64_t)sizeof(TO) > kStreamBytes) return sum_ids<T, TO, false, true>(ctx, stream, dE, dy, vals, scale, p);
   return sum_ids<T, TO, false, false>(ctx, stream, dE, dy, vals, scale, p);
@@ -298,7 +304,7 @@ int launch_experts(futhark_context *ctx, const char *who, hipStream_t stream, TO
     g.split = ctx->num_cu;
     blocks += cdiv(ctx->num_cu / 2, kXcds) * kXcds + 4 * kXcds;
   }
-  SAMD_TRY(check_blocks(ctx, who, blocks));
+  SAMD_TRY(check_row(ctx, who, blocks, WM * WN * kWave));
   g.m_tiles = (int)m_tiles;
   g.n_tiles = (int)n_tiles;
   if constexpr (KERNEL == kFew)
@@ -481,6 +487,9 @@ int sparse_amd_tokens_lookup_grad(struct futhark_context *ctx, void *stream, int
         // it is written before the last of what is read has been
         SAMD_TRY(check_panels(ctx, who, 1, {{"the workspace", work, 1, p.bytes, p.bytes, 1}, {"dy", dy, n, D, ldy, (int64_t)sizeof(T)},
                                             {"ids", ids, 1, n, n, (int64_t)sizeof(I)}, {"vals", vals, 1, vals ? n : 0, n, 4}}));
+        if (!accumulate) p.zero(out_type);
+        SAMD_TRY(check_blocks(ctx, who, p.sum_blocks()));
+        SAMD_TRY(check_blocks(ctx, who, p.join_blocks()));
         SAMD_TRY(order_ids<I>(ctx, s, (const I *)ids, p, !accumulate));
         if (out_type == type) return sum_ids_as<T, T>(ctx, s, accumulate != 0, (T *)dtable, (const T *)dy, vals, scale, p);
         return sum_ids_as<T, float>(ctx, s, accumulate != 0, (float *)dtable, (const T *)dy, vals, scale, p);

@@ -99,8 +99,20 @@ __device__ __forceinline__ int lane_id() { return (int)(threadIdx.x & (kWave - 1
 // The same in every lane of a wave, and known to be: what is indexed by it is loaded once per wave.
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave)); }
 
+// A grid holds fewer than 2^32 threads along x.  A launch of more workgroups has several rows of kGridRow of them (of up to 1024
+// threads), the last row whole as well: a kernel returns for a number behind its last one.
+constexpr int kGridRowLog = 21;
+constexpr int64_t kGridRow = (int64_t)1 << kGridRowLog;
+
+inline dim3 grid_of(int64_t blocks, int threads) {
+  if (blocks * threads < (int64_t)1 << 32) return dim3((unsigned)blocks);
+  return dim3((unsigned)kGridRow, (unsigned)cdiv(blocks, kGridRow));
+}
+
+__device__ __forceinline__ int64_t block_number() { return ((int64_t)blockIdx.y << kGridRowLog) + blockIdx.x; }
+
 // Among the waves of a launch of kThreads threads a workgroup.
-__device__ __forceinline__ int64_t wave_number() { return (int64_t)blockIdx.x * kWaves + wave_id(); }
+__device__ __forceinline__ int64_t wave_number() { return block_number() * kWaves + wave_id(); }
 
 // How a launch deals rows to waves.  Rows of 64 pieces or more: a wave takes `u` x 64 pieces of one row, `segs` waves a
 // row.  Shorter rows: a power of two of lanes each (1 << lg), so that a wave takes several.

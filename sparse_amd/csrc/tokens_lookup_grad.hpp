@@ -40,7 +40,7 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_kernel(TO *__restrict__ 
                                                                const uint8_t *__restrict__ named, float *__restrict__ part,
                                                                GradShape g) {
   constexpr int R = 8;
-  const int64_t w = (int64_t)blockIdx.x * kWaves + wave_id();
+  const int64_t w = wave_number();
   const int lane = lane_id();
   const int64_t chunk = w / g.segs;
   if (chunk >= g.chunks) {  // zero the rows no id names (named: a byte for each row)
@@ -113,7 +113,7 @@ template <class T, class TO, bool ADD, bool STREAM>
 __global__ __launch_bounds__(kThreads) void lookup_grad_join_kernel(TO *__restrict__ dE, const uint32_t *__restrict__ keys,
                                                                     float *__restrict__ part, GradShape g) {
   __shared__ float sums[kWaves][kWave][kPer<T>];
-  const int64_t chunk = blockIdx.x / g.segs;
+  const int64_t chunk = block_number() / g.segs;
   const int64_t p0 = chunk * g.chunk, p1 = p0 + g.chunk;
   if (p1 >= g.n) return;
   const uint32_t run = keys[p1 - 1];
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(kThreads) void lookup_grad_join_kernel(TO *__restri
   }
   const int64_t each = (count + kWaves - 1) / kWaves;
   const int64_t k0 = wave_id() * each, k1 = k0 + each < count ? k0 + each : count;
-  const int64_t unit = (blockIdx.x - chunk * g.segs) * kWave + lane_id();
+  const int64_t unit = (block_number() - chunk * g.segs) * kWave + lane_id();
   const int64_t c = unit * kPer<T>;
   float s[kPer<T>] = {};
   if (c < g.D) {

@@ -53,7 +53,7 @@ template <class T, class I>
 __global__ __launch_bounds__(kThreads) void lookup_dots_kernel(float *__restrict__ df, const T *__restrict__ dy, int64_t ldy,
                                                                const T *__restrict__ E, int64_t ldE, int64_t V, int64_t D,
                                                                const I *__restrict__ ids, int64_t n, float scale) {
-  const int64_t row = (int64_t)blockIdx.x * kWaves + wave_id();
+  const int64_t row = wave_number();
   if (row >= n) return;
   const int64_t id = (int64_t)ids[row];
   float s = 0.0f;
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(kThreads) void combine_grad_kernel(T *__restrict__ 
                                                                 int64_t slots, const float *__restrict__ w) {
   static_assert(W == 1 || W == kWaves, "a token has a wave or a workgroup");
   __shared__ float part[kWaves][J];
-  const int64_t t = W == 1 ? (int64_t)blockIdx.x * kWaves + wave_id() : blockIdx.x;
+  const int64_t t = W == 1 ? wave_number() : block_number();
   if (t >= n) return;
   const int first = W == 1 ? lane_id() : (int)threadIdx.x;
   for (int j0 = 0; j0 < K; j0 += J) {

@@ -524,6 +524,58 @@ def test_far_rows(tk):
     assert (W[4, -1, 5] == 4.0) and not W[4, -2].any() and not W[0].any()
 
 
+# 2^26 and a few rows, a wave each: more threads than the first dimension of a grid can have.  What is read is one row for all
+# of them, what is written (35 GB) has a different value in every few rows.
+MANY = (1 << 26) + 6
+
+
+def every_row_is(out, value):
+    """All columns of row i are value[i], looked at in parts."""
+    step = 1 << 22
+    return all(bool((out[i:i + step] == value[i:i + step, None]).all()) for i in range(0, len(out), step))
+
+
+@pytest.mark.parametrize("op", ["lookup", "dispatch", "combine", "combine_grad", "combine_grad wide", "lookup_vals_grad", "lookup_grad"])
+def test_more_rows_than_a_grid_has_in_a_row(tk, op):
+    k, n = tk("bf16"), MANY if op != "combine_grad wide" else (1 << 24) + 6
+    torch.cuda.empty_cache()
+    one = lambda D, n=n: torch.ones(1, D, device="cuda", dtype=torch.bfloat16).expand(n, D)  # noqa: E731
+    v = torch.arange(n, device="cuda", dtype=torch.int32) % 251     # exact in 8 bits
+    zero = torch.zeros(n, device="cuda", dtype=torch.int32)
+    if op == "lookup":
+        assert every_row_is(k.lookup(one(264, 1), zero, vals=v.float()), v)
+    elif op == "lookup_vals_grad":
+        assert torch.equal(k.lookup_vals_grad(v.bfloat16()[:, None], one(1, 1), zero, scale=2.0), 2.0 * v)
+    elif op == "lookup_grad":                                       # nearly all of it is zeros
+        ids = torch.arange(300, device="cuda") * (n // 300)
+        ids[-1] = n - 1
+        got = k.lookup_grad(one(264, 300), ids, n)
+        want = torch.zeros(n, device="cuda").index_fill_(0, ids, 1.0)
+        assert every_row_is(got, want)
+    else:
+        r = k.route(zero[:, None], 1)
+        if op == "dispatch":
+            assert every_row_is(k.dispatch(one(264), r, v.float()[:, None]), v)
+        elif op == "combine":
+            assert every_row_is(k.combine(one(264), r, v.float()[:, None]), v)
+        else:
+            D = 1 if op == "combine_grad" else 1040
+            dys, dw = k.combine_grad(one(D), one(D), r, v.float()[:, None])
+            assert every_row_is(dys, v) and bool((dw == D).all())
+    torch.cuda.empty_cache()
+
+
+def test_more_parts_of_runs_than_a_grid_has_in_a_row(tk):
+    """2^29 ids and a few: a workgroup for every 32 of them joins the sums that cross parts.  Sums of ones stay exact."""
+    k, n, V = tk("bf16"), (1 << 29) + 70, 1000
+    torch.cuda.empty_cache()
+    ids = torch.arange(n, device="cuda", dtype=torch.int32) % V
+    got = k.lookup_grad(torch.ones(1, 1, device="cuda", dtype=torch.bfloat16).expand(n, 1), ids, V, dtype=torch.float32)
+    assert torch.equal(got[:, 0], (n // V + (torch.arange(V, device="cuda") < n % V)).float())
+    del ids, got
+    torch.cuda.empty_cache()
+
+
 # ------------------------------------------------------------------------------------------------ gradients against differences
 def test_gradients_are_the_differences(tk):
     """Every operator is linear in each argument: with small whole numbers nothing is rounded, and a difference over a step

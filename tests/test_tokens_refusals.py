@@ -99,6 +99,13 @@ def test_combine_grad_and_grad_x_refuse_overlaps(call):
     assert rc != 0 and "overlaps" in text
 
 
+# a grid has fewer than 2^32 threads in its first dimension: tiles of 512 threads reach that before their number does
+@pytest.mark.parametrize("rows,words", [(1 << 22, "no usable HIP device"), (1 << 24, "more work than one launch"), (1 << 30, "more work than one launch")])
+def test_a_launch_of_tiles_too_many_is_refused(call, rows, words):
+    rc, text = experts(call, ys=1 << 58, ldy=1 << 16, xs=1 << 44, rows=rows, X=1, F=1 << 16)
+    assert rc != 0 and words in text, text
+
+
 # the workspace is written while the inputs are still read; where none is needed, what is given for one is not touched
 @pytest.mark.parametrize("f,change,words", [(grad, dict(n=300, work=B), "workspace overlaps dy"), (grad, dict(n=300, dy=W - 300 * 128 + 128, work=W), "workspace overlaps dy"),
                                             (grad, dict(n=300, work=C), "workspace overlaps ids"), (grad, dict(n=300, vals=D + 512, work=D), "workspace overlaps vals"),
