@@ -243,6 +243,8 @@ class mk_tokens:
     def _routing(self, r):
         if not isinstance(r, Routing):
             raise SparseError("expected a Routing (the result of route)")
+        if r._buf.get_device() != self._dev:
+            raise SparseError("the routing: expected one on cuda:%d" % self._dev)
         return r
 
     def _weights(self, w, r):

@@ -153,3 +153,20 @@ def test_the_python_side_refuses_what_is_not_on_the_device():
         tk.combine(E_, ids)
     with pytest.raises(AssertionError):
         mk_tokens("f64", Ctx())
+
+
+@pytest.mark.parametrize("name", ["dispatch", "combine", "dispatch_grad", "combine_grad", "experts", "experts_grad_x", "experts_grad_w"])
+def test_a_routing_of_another_device_is_refused(name):
+    """Its addresses are another device's: every operator that takes one looks where it is before anything else."""
+    import torch
+    from sparse_amd.compressed import SparseError
+    from sparse_amd.tokens import Routing, mk_tokens
+
+    class Ctx:
+        L, h, device = load_library(), None, 0
+    buf = torch.zeros(2 * 4 + 4, dtype=torch.int32)
+    r = Routing(buf, buf.data_ptr(), 2, 2, 3)
+    a = torch.zeros(4, 8, dtype=torch.bfloat16)
+    args = {"combine_grad": (a, a, r, None), "experts": (a, a, r), "experts_grad_x": (a, a, r), "experts_grad_w": (a, a, r)}.get(name, (a, r))
+    with pytest.raises(SparseError, match="routing: expected one on cuda:0"):
+        getattr(mk_tokens("bf16", Ctx()), name)(*args)
