@@ -33,6 +33,7 @@ import torch
 from .compressed import SparseError, default_context
 
 _VP, _I64, _INT, _F32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+_MAX_EXPERTS, _MAX_ROWS = 1024, 2 ** 31 - 2      # as the library has them: refused before a result of such a size is allocated
 _TYPES = {"f32": (0, torch.float32), "f16": (1, torch.float16), "bf16": (2, torch.bfloat16)}
 
 _SIGNATURES = {
@@ -201,10 +202,10 @@ class mk_tokens:
         32 bits in an order that the ids alone decide.  dy: [ids.numel(), D] (or ids.shape + (D,), contiguous).  accumulate: added to
         `out` instead of written over it; rows no id names are then not touched.  dtype (without `out`): the module's
         element type or torch.float32."""
-        i, bits, n = self._ids(ids, "ids")
         V = int(V)
-        if V < 0:
-            raise SparseError("lookup_grad: %d rows" % V)
+        if V < 0 or V > _MAX_ROWS:
+            raise SparseError("lookup_grad: %d rows (0 to %d are offered)" % (V, _MAX_ROWS))
+        i, bits, n = self._ids(ids, "ids")
         g, ldg, _, D = self._panel(self._as_rows(dy, ids), "dy", rows=n)
         f = self._floats(vals, "vals", ids.shape) if vals is not None else None
         if accumulate and out is None:
@@ -230,9 +231,11 @@ class mk_tokens:
         """Places for the experts that each token chose: chosen[tokens, K], 0 .. X-1 (anything else: no place)."""
         if isinstance(chosen, torch.Tensor) and chosen.dim() != 2:
             raise SparseError("chosen: expected 2 dimensions, got %d" % chosen.dim())
-        c, bits, n = self._ids(chosen, "chosen")
         X = int(X)
-        buf = torch.empty(2 * n + max(X, 0) + 1, dtype=torch.int32, device=self._device)
+        if X < 1 or X > _MAX_EXPERTS:
+            raise SparseError("route: %d experts (1 to %d are offered)" % (X, _MAX_EXPERTS))
+        c, bits, n = self._ids(chosen, "chosen")
+        buf = torch.empty(2 * n + X + 1, dtype=torch.int32, device=self._device)
         size = self._c_route_work(n, X)
         w, wp = self._scratch(size)
         p = buf.data_ptr()

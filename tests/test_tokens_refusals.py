@@ -170,3 +170,19 @@ def test_a_routing_of_another_device_is_refused(name):
     args = {"combine_grad": (a, a, r, None), "experts": (a, a, r), "experts_grad_x": (a, a, r), "experts_grad_w": (a, a, r)}.get(name, (a, r))
     with pytest.raises(SparseError, match="routing: expected one on cuda:0"):
         getattr(mk_tokens("bf16", Ctx()), name)(*args)
+
+
+@pytest.mark.parametrize("X", [-1, 0, 1025, 2 ** 40, 2 ** 64 + 4])
+def test_too_many_experts_or_rows_are_refused_before_they_are_allocated(X):
+    import torch
+    from sparse_amd.compressed import SparseError
+    from sparse_amd.tokens import mk_tokens
+
+    class Ctx:
+        L, h, device = load_library(), None, 0
+    tk, ids = mk_tokens("bf16", Ctx()), torch.zeros(2, 2, dtype=torch.int64)
+    with pytest.raises(SparseError, match="experts"):
+        tk.route(ids, X)
+    if X < 0 or X > 2 ** 31:
+        with pytest.raises(SparseError, match="rows"):
+            tk.lookup_grad(torch.zeros(4, 8, dtype=torch.bfloat16), ids, X)
