@@ -619,7 +619,8 @@ int sparse_amd_dcsr_f64_smvm(struct sparse_amd_group *g, struct sparse_amd_dvec_
  *     Sums are held in 32 bits and rounded once; values, weights and their gradients are 32-bit floats;
  *   - indices that come in have `id_bits` = 32 or 64 bits.  An id outside 0 .. V-1, or an expert outside 0 .. X-1, selects
  *     nothing: a row of zeros, no place (pos = -1), no gradient;
- *   - results are the same bits on every call with the same arguments;
+ *   - results are the same bits on every call with the same arguments.  A row of an experts' product may differ in its last
+ *     bits where the other rows of the batch differ: they decide which workgroup adds it, and where it begins;
  *   - a result may not overlap another result or an argument, nor lie between its rows.
  * Errors: as everywhere in this header (non-zero, text in futhark_context_get_error); nothing is launched then. */
 #define SPARSE_AMD_F32 0
@@ -633,8 +634,8 @@ int sparse_amd_tokens_lookup(struct futhark_context *ctx, void *stream, int type
 int sparse_amd_tokens_lookup_dots(struct futhark_context *ctx, void *stream, int type, float *dvals, const void *dy,
                                   int64_t ldy, const void *table, int64_t V, int64_t D, int64_t ldt, const void *ids,
                                   int id_bits, int64_t n, float scale);
-/* dtable[v] = sum over i with ids[i] = v of scale vals[i] dy[i], added in an order that the ids alone decide: lookup's gradient
- * by the table.
+/* dtable[v] = sum over i with ids[i] = v of scale vals[i] dy[i], added in an order that the ids, their number, the type and the
+ * width decide: lookup's gradient by the table.
  * accumulate = 0: every row of dtable is written (zeros where no id names it); else the sums are added to dtable, and rows
  * no id names are not touched.  out_type: type or SPARSE_AMD_F32.  V and n are at most 2^31 - 2. */
 int sparse_amd_tokens_lookup_grad(struct futhark_context *ctx, void *stream, int type, int out_type, int accumulate,

@@ -11,9 +11,13 @@
 // with the expert's last row (its last chunk of 16 bytes), so what a ragged tile would read beyond it is zero and costs no
 // memory access.
 //
-// What bounds it: with few rows an expert the blocks' bytes (32 blocks of 4096 x 2048, 4 rows each: 77 us, 7.0 TB/s), with many the
-// matrix cores' clock under power: 2048 rows each, 1220 TFLOP/s forward and 1140 for the gradient by xs, where a large
-// library product reaches 1430 to 1520.
+// What bounds it: with few rows an expert the blocks' bytes (32 blocks of 4096 x 2048, 2 rows each: 75 us, 7.2 TB/s), with many the
+// matrix cores and what they wait for at a tile's ends: 8 blocks of 4096 x 4096, 2048 rows each, 1380 to 1400 TFLOP/s forward,
+// 1360 by xs, 1347 by W; 16 of 4096 x 2048, 1024 rows each, whose tiles have half the steps or fewer, 1220 to 1250, 1250 and
+// 1156.  A library product of as many operations reaches 1520 to 1590.
+//
+// Forward, the order in which a row's products are added depends on the workgroup that its tile falls to: a row's last bits
+// may change with the other rows of the batch, though not from call to call.
 //
 // LDS layouts.  "Lying" operands (summed index side by side): row r is a step's slice, its 16-byte chunks permuted by a
 // function of r; a fragment is one ds_read_b128.  "Standing" operands (summed index down the rows): row k is R elements,
@@ -649,7 +653,7 @@ __global__ __launch_bounds__(WM *WN *kWave, 4) void experts_few_kernel(TO *__res
 // waits count the loads that a barrier later all waves may need.
 //
 // Four stages of 32, as above but in turns, take 64 bytes of a lying operand's row at a time: 16 experts of 4096 x 2048,
-// 1024 rows each, forward: 1202 TFLOP/s, in steps of 64 1291; the other two products, 1295 and 1306, are as fast either way.
+// 1024 rows each, forward: 7 % slower than steps of 64 where both were timed in turn; the other two products are as fast either way.
 template <class T>
 struct Parts {  // [of the even and the odd steps]; an array each: what is read from one does not wait for loads into another
   T *up0, *up1, *low0, *low1, *col0, *col1;

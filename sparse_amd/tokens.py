@@ -14,13 +14,14 @@ Neighbours of sparse_amd.mono (a record of col_idx[n] and vals[n], mono.fut:95) 
 call is one entry of include/sparse_amd.h, group (7), where the formulas stand.  What differs from the other modules:
 
 * arguments and results are torch CUDA tensors (numpy knows no bf16), on the context's device; a row of a panel is
-  contiguous, its rows may be any stride apart (expanded rows too, where they are only read);
+  contiguous, its rows may be any stride apart (expanded rows too, where they are only read).  Ids, choices, values and
+  weights are contiguous;
 * a call runs on torch's current stream of that device, like torch's own operations, whatever stream the context is on; it
   allocates from torch's allocator only, never waits, and may be captured into a graph.  Rows of a result it does not
   define (behind the last routed slot) are whatever the memory held, or what `out` held;
 * an id or an expert out of range selects nothing (row of zeros, place -1); there is no error for it, since that would
   have to wait for the device;
-* `out` shares no memory with an argument;
+* `out` shares no memory with an argument, and does not lie between an argument's rows;
 * nothing is recorded for torch's autograd: the gradients are calls of their own.
 
 Arguments that do not fit (type, shape, device, overlap) raise SparseError before anything is launched.
@@ -199,7 +200,7 @@ class mk_tokens:
 
     def lookup_grad(self, dy, ids, V, vals=None, scale=1.0, out=None, accumulate=False, dtype=None):
         """lookup's gradient by the table: dE[v] = the sum of scale * vals[i] * dy[i] over the i with ids[i] = v, added in
-        32 bits in an order that the ids alone decide.  dy: [ids.numel(), D] (or ids.shape + (D,), contiguous).  accumulate: added to
+        32 bits in an order that the ids, their number, the type and D decide.  dy: [ids.numel(), D] (or ids.shape + (D,), contiguous).  accumulate: added to
         `out` instead of written over it; rows no id names are then not touched.  dtype (without `out`): the module's
         element type or torch.float32."""
         V = int(V)
@@ -304,7 +305,8 @@ class mk_tokens:
         return W.data_ptr(), F, D, ld if F > 1 or ld > D else D, block
 
     def experts(self, xs, W, r, out=None):
-        """ys[p] = W[e] xs[p] for every expert e's places p: [slots, F] from xs[slots, D], W[X, F, D]."""
+        """ys[p] = W[e] xs[p] for every expert e's places p: [slots, F] from xs[slots, D], W[X, F, D].  A row's last bits may
+        depend on the other rows of the batch, not on the call."""
         r = self._routing(r)
         w, F, D, ldw, block = self._blocks(W, "W", r.X)
         a, lda, n, _ = self._panel(xs, "xs", rows=r.slots, cols=D)
