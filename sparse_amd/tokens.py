@@ -63,11 +63,11 @@ class Routing:
     """Where a batch's choices go (tk.route).  pos[tokens, K]: the place of every choice, -1 where it names no expert;
     src[tokens * K]: the choice (token * K + j) at every place, -1 behind the last; offsets[X + 1]: expert e has the places
     offsets[e] .. offsets[e + 1] - 1.  All int32, on the device, in one buffer."""
-    __slots__ = ("tokens", "K", "X", "slots", "_buf", "_pos", "_offsets")
+    __slots__ = ("tokens", "K", "X", "slots", "_buf", "_pos", "_offsets", "_on")
 
     def __init__(self, buf, address, tokens, K, X):
         self.tokens, self.K, self.X, self.slots = tokens, K, X, tokens * K
-        self._buf, self._pos, self._offsets = buf, address, address + 8 * tokens * K
+        self._buf, self._pos, self._offsets, self._on = buf, address, address + 8 * tokens * K, buf.get_device()
 
     @property
     def pos(self):
@@ -247,7 +247,7 @@ class mk_tokens:
     def _routing(self, r):
         if not isinstance(r, Routing):
             raise SparseError("expected a Routing (the result of route)")
-        if r._buf.get_device() != self._dev:
+        if r._on != self._dev:
             raise SparseError("the routing: expected one on cuda:%d" % self._dev)
         return r
 
